@@ -29,7 +29,7 @@
 //    of global atomics into the [P][16] accumulator.
 #include "render_common.h"
 
-typedef float v2f __attribute__((ext_vector_type(2)));  // pairs of channels go through the packed-FP32 instructions
+typedef float v2f __attribute__((ext_vector_type(2)));  // pairs of channels, written once (the build turns packed FP32 off)
 
 // One step of the reduce-scatter inside a 16-lane row.  `ctrl` is a DPP pattern that pairs every lane with a lane
 // whose `upper` flag is the opposite; afterwards the lanes with upper == false hold a summed over each pair, the
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(NGS_TILE_PIX, 6) void render_bwd_kernel(
         auto step = [&](const int it, const int j, const float4 p, const float4 q, const float4 col, const bool shared) {
             const bool have = it < my_n;
             // same evaluation order as the forward pass (and the reference): alpha must come out bit-identical;
-            // the two squares as a pair (packed FP32: same roundings, half the issue slots)
+            // the two squares written as a pair
             const v2f d = (v2f){p.x, p.y} - pix;
             const v2f sq = ((v2f){p.z, p.w} * d) * d;  // {a dx dx, c dy dy}
             const float dx = d.x, dy = d.y;

@@ -122,7 +122,7 @@ __global__ __launch_bounds__(NGS_TILE_PIX, NGS_FWD_WG_PER_CU) void render_fwd_ke
     uint32_t last_contributor = 0;
 
     // One entry of a row's list: the splat in the slot at LDS address `at` against the row's 16 pixels.  The two
-    // squares of the exponent are formed as pairs (packed FP32 instructions: same roundings, half the issue slots).
+    // squares of the exponent are written as pairs.
     const fwd_f2 pix = {pxf, pyf};
     auto visit = [&](const uint32_t at) {
         const fwd_f4 p = fwd_lds_read<fwd_f4>(at), q = fwd_lds_read<fwd_f4>(at + 16);
