@@ -407,6 +407,76 @@ int ngs_idxmap_forward_static(int P, int width, int height, const float* means3D
                               int* num_rendered_device, void* stream);
 
 /*
+ * Operators over feature rows: what a decoder of the index map's feature rows (above) is built from.  The reference
+ * leaves its decoders to torch's operators (utils/net_utils.py); these have no native counterpart there.
+ *
+ * dtype names the element type of every array typed void* unless noted.  Row strides are in elements and may be any
+ * non-negative number; elements of a row are contiguous, and so are outputs, rows included.  Arrays need the
+ * alignment of their element type only; a workspace needs 16 bytes.  Sums, statistics and activations are formed in
+ * 32 bits, each output is rounded once, and results do not depend on timing (no atomics).  Sizes of zero are fine.
+ * Outputs must not overlap inputs, unless noted.
+ *
+ * ngs_linear_forward: y = act(x weight^T + bias) + residual, with x [rows][in_features] (rows x_stride apart), weight
+ * [out_features][in_features] (rows weight_stride apart), bias [out_features] or NULL, residual [rows][out_features]
+ * (rows residual_stride apart) or NULL, y [rows][out_features].  GELU is x Phi(x), SILU x sigmoid(x).  slope, if not
+ * NULL, receives the activation's derivative at every element, [rows][out_features], for the backward pass: floats
+ * for NGS_FLOAT32, half precision (NGS_FLOAT16) for both 16-bit types -- the derivative is bounded, so its 11 bits
+ * are finer than the types' own rounding of the gradient.  NGS_ACT_NONE needs none and writes none.
+ *
+ * ngs_linear_backward: with dz = dL_dy * slope, dL_dx = dz weight, dL_dweight = dz^T x, dL_dbias = sum of dz over the
+ * rows; any of the three may be NULL.  dL_dy [rows][out_features], rows dL_dy_stride apart.  (A residual's gradient
+ * is dL_dy itself.)  For the 16-bit types dz is rounded to the type in front of the two products, which the matrix
+ * units take in that type; dL_dbias sums it unrounded.
+ *
+ * ngs_layer_norm_forward: y = (x - m) r weight + bias with m the mean of a row of x [rows][width] and
+ * r = 1 / sqrt(variance + eps), the variance the biased one about m.  weight and bias [width] are of weight_dtype
+ * (dtype or NGS_FLOAT32), either may be NULL (ones, zeros).  mean and rstd [rows], floats, may be NULL: the backward
+ * pass reads them.
+ * ngs_layer_norm_backward: with g = dL_dy weight and u = (x - m) r,
+ * dL_dx = r (g - mean g - u mean(g u)), dL_dweight = sum over rows of dL_dy u, dL_dbias = sum of dL_dy; any may be
+ * NULL.  The last two are of weight_dtype.
+ *
+ * ngs_dropout: y = residual + (kept ? x * 65536 / (65536 - t) : 0), t = p * 65536 rounded to the nearest whole number
+ * (p in [0, 1]; with t = 65536 nothing is kept).  Element i (counted along the rows of the [rows][cols] array,
+ * whatever the strides) is kept if the 16-bit half i % 8 (low half of a word first) of block i / 8 of the
+ * Philox 4x32 generator with 7 rounds is at least t; the key is `seed`, the counter (block, offset): one offset for
+ * each use of a seed gives unrelated masks.  seed_device, if not NULL, is a device address of the seed, which is read
+ * when the kernel runs (a captured graph gets new masks by changing it).  No mask is stored: the backward pass is the same call on dL_dy, without a
+ * residual.  What is dropped becomes zero even if it is infinite or NaN.  y may be x or residual itself (same rows,
+ * same strides).
+ */
+#define NGS_FLOAT32 0
+#define NGS_FLOAT16 1
+#define NGS_BFLOAT16 2
+#define NGS_ACT_NONE 0
+#define NGS_ACT_RELU 1
+#define NGS_ACT_GELU 2
+#define NGS_ACT_SILU 3
+#define NGS_ACT_SIGMOID 4
+size_t ngs_linear_forward_workspace_bytes(long long rows, int in_features, int out_features, int dtype);
+int ngs_linear_forward(long long rows, int in_features, int out_features, int dtype, int activation, const void* x,
+                       long long x_stride, const void* weight, long long weight_stride, const void* bias,
+                       const void* residual, long long residual_stride, void* y, void* slope, char* workspace,
+                       void* stream);
+size_t ngs_linear_backward_workspace_bytes(long long rows, int in_features, int out_features, int dtype,
+                                           int activation);
+int ngs_linear_backward(long long rows, int in_features, int out_features, int dtype, int activation, const void* x,
+                        long long x_stride, const void* weight, long long weight_stride, const void* slope,
+                        const void* dL_dy, long long dL_dy_stride, void* dL_dx, void* dL_dweight, void* dL_dbias,
+                        char* workspace, void* stream);
+int ngs_layer_norm_forward(long long rows, int width, int dtype, int weight_dtype, float eps, const void* x,
+                           long long x_stride, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                           void* stream);
+size_t ngs_layer_norm_backward_workspace_bytes(long long rows, int width, int dtype);
+int ngs_layer_norm_backward(long long rows, int width, int dtype, int weight_dtype, const void* x, long long x_stride,
+                            const void* weight, const float* mean, const float* rstd, const void* dL_dy,
+                            long long dL_dy_stride, void* dL_dx, void* dL_dweight, void* dL_dbias, char* workspace,
+                            void* stream);
+int ngs_dropout(long long rows, long long cols, int dtype, double p, unsigned long long seed,
+                const unsigned long long* seed_device, unsigned long long offset, const void* x, long long x_stride,
+                const void* residual, long long residual_stride, void* y, void* stream);
+
+/*
  * Scene initialisation: mean_dist2[i] = mean of the squared distances from point i to its three nearest other
  * points = SimpleKNN::knn (submodules/simple-knn/simple_knn.h:16-19, simple_knn.cu:185-221), the routine behind
  * simple_knn._C.distCUDA2 (spatial.cu:15-26, ext.cpp:15-17), whose result scene/gaussian_model.py:160-161 turns into

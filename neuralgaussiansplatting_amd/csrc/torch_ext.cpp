@@ -15,6 +15,10 @@
 
 #include "../../include/ngs_rasterizer.h"
 
+// torch_decoder.cpp
+void ngs_decoder_bind(void* handle, const std::string& path);
+void ngs_decoder_register(pybind11::module_& m);
+
 namespace {
 
 struct Api {
@@ -48,6 +52,7 @@ void bind(const std::string& path)
     resolve(api.backward, "ngs_rasterize_backward", path);
     resolve(api.mark_visible, "ngs_mark_visible", path);
     resolve(api.last_error, "ngs_last_error", path);
+    ngs_decoder_bind(h, path);
 }
 
 void require_bound() { TORCH_CHECK(api.handle != nullptr, "the rasterizer library has not been bound (call bind(path) first)"); }
@@ -231,6 +236,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("mark_visible", &mark_visible, py::arg("means3D"), py::arg("viewmatrix"), py::arg("projmatrix"));
     m.def("bind", &bind, py::arg("library_path"),
           "Load libngs_rasterizer.so from this path and resolve the entry points the three functions call.");
+    ngs_decoder_register(m);
     m.def("set_forced_binning_capacity", &set_forced_binning_capacity, py::arg("capacity"),
           "Tests: a capacity >= 0 replaces the estimate of the binning buffer's size (0 = wait for the count); -1 "
           "restores the estimate.");
