@@ -102,8 +102,7 @@ inline int ngs_decoder_operand(const char* what, const void* p, long long rows, 
     return 0;
 }
 
-// Joins workgroups' sums of columns, always in the same order: out0[c] = sum over b of partial[b][c].  With out1 the
-// rows of `partial` are two widths long and the second half goes to out1.  A NULL output is left out (out1 NULL with
-// `halves` 2: rows are two widths long all the same).  No rows: zeros.
-void ngs_launch_column_finish(hipStream_t s, const float* partial, long long blocks, long long width, int halves, void* out0,
-                              void* out1, int dtype);
+// Joins workgroups' sums of columns, always in the same order: out[c] = sum over b of partial[b][c], rows width0 + width1
+// long, the first width0 columns going to out0, the others to out1.  A NULL output is left out.  No rows: zeros.
+void ngs_launch_column_finish(hipStream_t s, const float* partial, long long blocks, long long width0, long long width1,
+                              void* out0, void* out1, int dtype);

@@ -407,7 +407,7 @@ static int norm_backward(hipStream_t st, int dtype, int weight_dtype, NormBackwa
     hipLaunchKernelGGL((norm_backward_kernel<T, W, G, C, THREADS>), dim3(blocks), dim3(THREADS), 0, st, a)
         NGS_NORM_DISPATCH(LAUNCH_BACKWARD)
     }
-    if (a.partial) ngs_launch_column_finish(st, a.partial, blocks, a.width, 2, dw, db, weight_dtype);
+    if (a.partial) ngs_launch_column_finish(st, a.partial, blocks, a.width, a.width, dw, db, weight_dtype);
     return ngs_decoder_launched("ngs_layer_norm_backward");
 }
 
@@ -459,7 +459,7 @@ extern "C" int ngs_layer_norm_backward(long long rows, int width, int dtype, int
     hipStream_t st = (hipStream_t)stream;
     const bool sums = dL_dweight || dL_dbias;
     if (rows == 0) {  // sums over nothing
-        if (sums) ngs_launch_column_finish(st, nullptr, 0, width, 2, dL_dweight, dL_dbias, weight_dtype);
+        if (sums) ngs_launch_column_finish(st, nullptr, 0, width, width, dL_dweight, dL_dbias, weight_dtype);
         return ngs_decoder_launched(what);
     }
     if (ngs_decoder_operand("ngs_layer_norm_backward: x", x, rows, width, x_stride) ||

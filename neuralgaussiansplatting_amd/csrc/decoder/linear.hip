@@ -8,106 +8,7 @@
 //   forward  P = W along,   Q = x along,   r = K
 //   dx       P = W across,  Q = dz along,  r = N
 //   dW       P = x across,  Q = dz across, r = M
-#include "decoder_common.h"
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-#define ROW_BYTES 128  // bytes of the reduction index that one step stages per row: 64 16-bit elements or 32 floats
-
-// Elements of the derivative array for T.
-template <typename T> struct Slope { typedef f16 type; };
-template <> struct Slope<float> { typedef float type; };
-
-// ---------------------------------------------------------------------------
-// Activations
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
-
-// act(z), and its derivative in `slope`
-__device__ __forceinline__ float activate(float z, int act, float& slope)
-{
-    slope = 1.0f;
-    if (act == NGS_ACT_RELU) {
-        slope = z > 0.0f ? 1.0f : 0.0f;
-        return z < 0.0f ? 0.0f : z;  // NaN stays
-    }
-    if (act == NGS_ACT_GELU) {
-        const float phi = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
-        slope = phi + z * (0.39894228040143268f * __expf(-0.5f * z * z));
-        return z * phi;
-    }
-    if (act == NGS_ACT_SILU) {
-        const float s = sigmoid(z);
-        slope = s * (1.0f + z * (1.0f - s));
-        return z * s;
-    }
-    if (act == NGS_ACT_SIGMOID) {
-        const float s = sigmoid(z);
-        slope = s * (1.0f - s);
-        return s;
-    }
-    return z;
-}
-
-// ---------------------------------------------------------------------------
-// What happens to four neighbouring sums of one result row
-// ---------------------------------------------------------------------------
-template <typename T>
-struct Epilogue {
-    int act;
-    int np;               // width of a result row
-    const T* bias;        // [np] or NULL
-    const T* residual;    // rows ldr apart, or NULL
-    long long ldr;
-    T* y;                 // [nq][np]
-    typename Slope<T>::type* slope;  // [nq][np] or NULL
-    float* partial;       // not NULL: the bare sums go to partial[split][q][p] and nothing else happens
-};
-
-template <typename U>
-__device__ __forceinline__ void store4(U* p, const float (&v)[4], int valid)
-{
-    union { U e[4]; } u;
-#pragma unroll
-    for (int i = 0; i < 4; i++) u.e[i] = (U)v[i];
-    if (valid >= 4) {
-        __builtin_memcpy(p, u.e, 4 * sizeof(U));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 3; i++)
-            if (i < valid) p[i] = u.e[i];
-    }
-}
-
-template <typename U>
-__device__ __forceinline__ void load4(const U* p, float (&v)[4], int valid)
-{
-    union { U e[4]; } u = {};
-    if (valid >= 4) {
-        __builtin_memcpy(u.e, p, 4 * sizeof(U));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 3; i++)
-            if (i < valid) u.e[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = (float)u.e[i];
-}
-
-template <typename T>
-__device__ __forceinline__ void finish4(const Epilogue<T>& e, long long q, int p, f32x4 z, const float (&bias)[4])
-{
-    const int valid = e.np - p;
-    const long long at = q * e.np + p;
-    float y[4], s[4], r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (e.residual) load4(e.residual + q * e.ldr + p, r, valid);
-#pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = activate(z[i] + bias[i], e.act, s[i]) + r[i];
-    store4(e.y + at, y, valid);
-    if (e.slope) store4(e.slope + at, s, valid);
-}
+#include "linear_common.h"
 
 // ---------------------------------------------------------------------------
 // The product kernel
@@ -122,101 +23,6 @@ struct Product {
     int splits;          // the reduction is cut into this many runs of `run` elements (a multiple of a step's)
     long long run;
     Epilogue<T> epi;
-};
-
-__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, const bf16*)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, const f16*)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c, const float*)
-{
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-    return c;
-}
-
-// One operand's tile of ROWS rows in shared memory, ROWS * ROW_BYTES bytes either way.
-//
-// Along: row after row, the eight 16-byte chunks of a row exchanged by the row's low bits, so that the 16 rows a
-// fragment is read from spread over the banks.  Lane (g, i) = (lane / 16, lane % 16) of a fragment holds row i,
-// chunk g of a group of four: 8 16-bit elements or 4 floats of the reduction.
-//
-// Across: one line of ROWS elements per reduction index.  A fragment needs, per lane, one column and neighbouring
-// reduction indices: 16-bit elements come through the transposing read (four lines of 16 columns per 16 lanes, two
-// reads a fragment), floats one by one.  The 16 columns' segment within the line is exchanged by the line's number,
-// so that the lines that are read together lie in different banks.
-template <typename T, bool ACROSS, int ROWS>
-struct Tile {
-    static constexpr int N = Chunk<T>::N;
-    static constexpr int STEP = ROW_BYTES / (int)sizeof(T);        // reduction elements of a step
-    static constexpr int CHUNKS = ROWS * (ROW_BYTES / 16);
-    static constexpr int LINE = ROWS * (int)sizeof(T) / 16;        // across: chunks of a line
-    static constexpr int SEG = (int)sizeof(T);                     // across: chunks of 16 columns (2 or 4)
-
-    static __device__ __forceinline__ int segment_swap(int line)
-    {
-        const int s = sizeof(T) == 2 ? (line & 3) | ((line >> 1) & 4) : (line >> 2) & 3;
-        return s & (LINE / SEG - 1);
-    }
-
-    // the 16 bytes that chunk number i of the tile holds, from memory
-    static __device__ __forceinline__ u32x4 fetch(const T* __restrict__ base, long long ld, long long row0,
-                                                  long long rows, long long r0, long long r_end, int i)
-    {
-        if (!ACROSS) {
-            const long long row = row0 + i / 8, r = r0 + (i % 8) * N;
-            if (row >= rows) return (u32x4){0, 0, 0, 0};
-            return load16_head(base + row * ld + r, r_end - r);
-        } else {
-            const long long r = r0 + i / LINE, col = row0 + (i % LINE) * N;
-            if (r >= r_end) return (u32x4){0, 0, 0, 0};
-            return load16_head(base + r * ld + col, rows - col);
-        }
-    }
-    static __device__ __forceinline__ void put(char* lds, int i, u32x4 v)
-    {
-        int at;
-        if (!ACROSS) {
-            const int row = i / 8, c = i % 8;
-            at = row * ROW_BYTES + ((c ^ (row & 7)) << 4);
-        } else {
-            const int line = i / LINE, c = i % LINE;
-            at = line * (LINE << 4) + ((c ^ (segment_swap(line) * SEG)) << 4);
-        }
-        *(u32x4*)(lds + at) = v;
-    }
-    // fragment of rows [16 block, 16 block + 16), half `s` of the step's reduction elements
-    static __device__ __forceinline__ u32x4 fragment(const char* lds, int block, int s, int lane)
-    {
-        const int g = lane >> 4, i = lane & 15;
-        if (!ACROSS) {
-            const int row = block * 16 + i, c = s * 4 + g;
-            return *(const u32x4*)(lds + row * ROW_BYTES + ((c ^ (row & 7)) << 4));
-        } else if (sizeof(T) == 2) {
-            const int line = s * 32 + g * 8 + (i >> 2);
-            const int seg = block ^ segment_swap(line);  // the same for line and line + 4
-            const char* at = lds + line * (LINE << 4) + (seg << 5) + ((i & 3) << 3);
-            typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * (LINE << 4)));
-            const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
-            return (u32x4){l.x, l.y, h.x, h.y};
-        } else {
-            u32x4 v;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int line = s * 16 + g * 4 + j;
-                const int seg = block ^ segment_swap(line);
-                v[j] = *(const uint32_t*)(lds + line * (LINE << 4) + (seg << 6) + (i << 2));
-            }
-            return v;
-        }
-    }
 };
 
 // A workgroup of WP x WQ waves computes a TP x TQ tile of one run of the reduction; each step's operands travel
@@ -376,37 +182,36 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long rows, int n, i
 // 16 columns by 64 rows of threads: a thread adds every 64th row, the 64 sums are joined pairwise.
 template <typename T>
 __global__ __launch_bounds__(1024) void column_finish_kernel(const float* __restrict__ partial, long long blocks,
-                                                             long long width, long long pitch, T* __restrict__ out0,
+                                                             long long width0, long long width1, T* __restrict__ out0,
                                                              T* __restrict__ out1)
 {
     __shared__ float sums[64][17];
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const long long c = (long long)blockIdx.x * 16 + tx;
-    T* const out = blockIdx.y ? out1 : out0;
-    if (!out) return;
+    const long long c = (long long)blockIdx.x * 16 + tx, pitch = width0 + width1;
     float s = 0.0f;
-    if (c < width)
-        for (long long b = ty; b < blocks; b += 64) s += partial[b * pitch + blockIdx.y * width + c];
+    if (c < pitch)
+        for (long long b = ty; b < blocks; b += 64) s += partial[b * pitch + c];
     sums[ty][tx] = s;
     __syncthreads();
     for (int half = 32; half > 0; half >>= 1) {
         if (ty < half) sums[ty][tx] += sums[ty + half][tx];
         __syncthreads();
     }
-    if (ty == 0 && c < width) out[c] = (T)sums[0][tx];
+    if (ty != 0 || c >= pitch) return;
+    T* const out = c < width0 ? out0 : out1;
+    if (out) out[c < width0 ? c : c - width0] = (T)sums[0][tx];
 }
 
-void ngs_launch_column_finish(hipStream_t s, const float* partial, long long blocks, long long width, int halves, void* out0,
-                              void* out1, int dtype)
+void ngs_launch_column_finish(hipStream_t s, const float* partial, long long blocks, long long width0, long long width1,
+                              void* out0, void* out1, int dtype)
 {
-    const dim3 grid((unsigned)((width + 15) / 16), (unsigned)halves), threads(1024);
-    const long long pitch = width * halves;
+    const dim3 grid((unsigned)((width0 + width1 + 15) / 16)), threads(1024);
     if (dtype == NGS_FLOAT32)
-        hipLaunchKernelGGL(column_finish_kernel<float>, grid, threads, 0, s, partial, blocks, width, pitch, (float*)out0, (float*)out1);
+        hipLaunchKernelGGL(column_finish_kernel<float>, grid, threads, 0, s, partial, blocks, width0, width1, (float*)out0, (float*)out1);
     else if (dtype == NGS_FLOAT16)
-        hipLaunchKernelGGL(column_finish_kernel<f16>, grid, threads, 0, s, partial, blocks, width, pitch, (f16*)out0, (f16*)out1);
+        hipLaunchKernelGGL(column_finish_kernel<f16>, grid, threads, 0, s, partial, blocks, width0, width1, (f16*)out0, (f16*)out1);
     else
-        hipLaunchKernelGGL(column_finish_kernel<bf16>, grid, threads, 0, s, partial, blocks, width, pitch, (bf16*)out0, (bf16*)out1);
+        hipLaunchKernelGGL(column_finish_kernel<bf16>, grid, threads, 0, s, partial, blocks, width0, width1, (bf16*)out0, (bf16*)out1);
 }
 
 // ---------------------------------------------------------------------------
@@ -523,14 +328,20 @@ static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtyp
     a.epi.ldr = ldr;
     a.epi.y = (T*)y;
     a.epi.slope = act == NGS_ACT_NONE ? nullptr : (typename Slope<T>::type*)slope;
+    a.epi.np = n;
+    if (ngs_stream_forward_takes(rows, k, n, dtype))
+        return ngs_stream_forward<T>(st, rows, k, n, dtype, a.q, ldx, a.p, ldw, a.epi);
     return launch_product<T, false, false>(st, product_shape(n, rows, k, dtype), a, (float*)workspace);
 }
 
 template <typename T>
 static int linear_backward(hipStream_t st, long long rows, int k, int n, int dtype, int act, const void* x, long long ldx,
-                           const void* w, long long ldw, const void* slope, const void* dy, long long lddy, void* dx,
-                           void* dw, void* db, char* workspace)
+                           const void* w, long long ldw, const void* bias, const void* slope, const void* dy, long long lddy,
+                           void* dx, void* dw, void* db, char* workspace)
 {
+    if (ngs_stream_backward_takes(rows, k, n, dtype))
+        return ngs_stream_backward<T>(st, rows, k, n, dtype, act, (const T*)x, ldx, (const T*)w, ldw, (const T*)bias,
+                                      (const T*)dy, lddy, (T*)dx, (T*)dw, (T*)db, (float*)workspace);
     const BackwardPlan b = backward_plan(rows, k, n, dtype, act);
     const T* dz = (const T*)dy;
     long long lddz = lddy;
@@ -542,7 +353,7 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
         hipLaunchKernelGGL(linear_dz_kernel<T>, grid, dim3(256), 0, st, rows, n, b.across, (const T*)dy, lddy,
                            act == NGS_ACT_NONE ? nullptr : (const typename Slope<T>::type*)slope,
                            make_dz ? (T*)workspace : nullptr, db ? sums : nullptr);
-        if (db) ngs_launch_column_finish(st, sums, b.row_blocks, n, 1, db, nullptr, dtype);
+        if (db) ngs_launch_column_finish(st, sums, b.row_blocks, n, 0, db, nullptr, dtype);
         if (ngs_decoder_launched("ngs_linear_backward")) return 1;
         if (make_dz) {
             dz = (const T*)workspace;
@@ -591,6 +402,7 @@ static int check_linear(const char* what, long long rows, int k, int n, int dtyp
 extern "C" size_t ngs_linear_forward_workspace_bytes(long long rows, int in_features, int out_features, int dtype)
 {
     if (rows <= 0 || out_features <= 0 || in_features < 0 || rows > (1LL << 40) || !ngs_decoder_dtype(dtype)) return 0;
+    if (ngs_stream_forward_takes(rows, in_features, out_features, dtype)) return 0;
     return product_shape(out_features, rows, in_features, dtype).partial_bytes(out_features, rows);
 }
 
@@ -620,17 +432,26 @@ extern "C" int ngs_linear_forward(long long rows, int in_features, int out_featu
                                 residual_stride, y, slope, workspace);
 }
 
+extern "C" int ngs_linear_backward_reads_slope(long long rows, int in_features, int out_features, int dtype, int activation)
+{
+    if (rows <= 0 || out_features <= 0 || !ngs_decoder_dtype(dtype) || activation == NGS_ACT_NONE) return 0;
+    return ngs_stream_backward_takes(rows, in_features, out_features, dtype) ? 0 : 1;
+}
+
 extern "C" size_t ngs_linear_backward_workspace_bytes(long long rows, int in_features, int out_features, int dtype,
                                                       int activation)
 {
     if (rows < 0 || in_features < 0 || out_features < 0 || rows > (1LL << 40) || !ngs_decoder_dtype(dtype)) return 0;
+    if (ngs_stream_backward_takes(rows, in_features, out_features, dtype))
+        return (size_t)ngs_stream_backward_blocks(rows, in_features, out_features, dtype) *
+               ((size_t)in_features * out_features + out_features) * sizeof(float);
     return backward_plan(rows, in_features, out_features, dtype, activation).total;
 }
 
 extern "C" int ngs_linear_backward(long long rows, int in_features, int out_features, int dtype, int activation,
                                    const void* x, long long x_stride, const void* weight, long long weight_stride,
-                                   const void* slope, const void* dL_dy, long long dL_dy_stride, void* dL_dx,
-                                   void* dL_dweight, void* dL_dbias, char* workspace, void* stream)
+                                   const void* bias, const void* slope, const void* dL_dy, long long dL_dy_stride,
+                                   void* dL_dx, void* dL_dweight, void* dL_dbias, char* workspace, void* stream)
 {
     const int k = in_features, n = out_features;
     if (check_linear("ngs_linear_backward", rows, k, n, dtype, activation)) return 1;
@@ -638,19 +459,21 @@ extern "C" int ngs_linear_backward(long long rows, int in_features, int out_feat
     if (n == 0 || k == 0) dL_dweight = nullptr;
     if (n == 0) dL_dbias = nullptr;
     if (!dL_dx && !dL_dweight && !dL_dbias) return 0;
-    if ((dL_dweight && ngs_decoder_operand("ngs_linear_backward: x", x, rows, k, x_stride)) ||
-        (dL_dx && ngs_decoder_operand("ngs_linear_backward: weight", weight, n, k, weight_stride)) ||
+    const bool reads_slope = ngs_linear_backward_reads_slope(rows, k, n, dtype, activation);
+    const bool forms_z = activation != NGS_ACT_NONE && !reads_slope;
+    if (((dL_dweight || forms_z) && ngs_decoder_operand("ngs_linear_backward: x", x, rows, k, x_stride)) ||
+        ((dL_dx || forms_z) && ngs_decoder_operand("ngs_linear_backward: weight", weight, n, k, weight_stride)) ||
         ngs_decoder_operand("ngs_linear_backward: dL_dy", dL_dy, rows, n, dL_dy_stride))
         return 1;
-    if (activation != NGS_ACT_NONE && ngs_decoder_operand("ngs_linear_backward: slope", slope, rows, n, n)) return 1;
+    if (reads_slope && ngs_decoder_operand("ngs_linear_backward: slope", slope, rows, n, n)) return 1;
     if (!workspace) return ngs_set_error("ngs_linear_backward: workspace", "is NULL");
     hipStream_t st = (hipStream_t)stream;
     if (dtype == NGS_FLOAT32)
-        return linear_backward<float>(st, rows, k, n, dtype, activation, x, x_stride, weight, weight_stride, slope, dL_dy,
+        return linear_backward<float>(st, rows, k, n, dtype, activation, x, x_stride, weight, weight_stride, bias, slope, dL_dy,
                                       dL_dy_stride, dL_dx, dL_dweight, dL_dbias, workspace);
     if (dtype == NGS_FLOAT16)
-        return linear_backward<f16>(st, rows, k, n, dtype, activation, x, x_stride, weight, weight_stride, slope, dL_dy,
+        return linear_backward<f16>(st, rows, k, n, dtype, activation, x, x_stride, weight, weight_stride, bias, slope, dL_dy,
                                     dL_dy_stride, dL_dx, dL_dweight, dL_dbias, workspace);
-    return linear_backward<bf16>(st, rows, k, n, dtype, activation, x, x_stride, weight, weight_stride, slope, dL_dy,
+    return linear_backward<bf16>(st, rows, k, n, dtype, activation, x, x_stride, weight, weight_stride, bias, slope, dL_dy,
                                  dL_dy_stride, dL_dx, dL_dweight, dL_dbias, workspace);
 }

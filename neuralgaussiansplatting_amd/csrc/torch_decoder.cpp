@@ -21,6 +21,7 @@ struct DecoderApi {
     decltype(&ngs_linear_forward_workspace_bytes) linear_forward_ws = nullptr;
     decltype(&ngs_linear_forward) linear_forward = nullptr;
     decltype(&ngs_linear_backward_workspace_bytes) linear_backward_ws = nullptr;
+    decltype(&ngs_linear_backward_reads_slope) linear_reads_slope = nullptr;
     decltype(&ngs_linear_backward) linear_backward = nullptr;
     decltype(&ngs_layer_norm_forward) norm_forward = nullptr;
     decltype(&ngs_layer_norm_backward_workspace_bytes) norm_backward_ws = nullptr;
@@ -142,10 +143,18 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                           int64_t act, const c10::optional<Tensor>& residual)
     {
         const bool gx = x.requires_grad(), gw = weight.requires_grad(), gb = wants_grad(bias);
+        const int64_t k = weight.size(1), n = weight.size(0);
+        int64_t rows = 1;
+        for (int64_t d = 0; d + 1 < x.dim(); d++) rows *= x.size(d);
+        const bool curved = act != NGS_ACT_NONE && (gx || gw || gb);
+        const bool keep = curved && api.linear_reads_slope(rows, (int)k, (int)n, dtype_of("linear", x), (int)act);
         Tensor slope;
-        Tensor y = linear_run(x, weight, bias, (int)act, residual, act != NGS_ACT_NONE && (gx || gw || gb) ? &slope : nullptr);
-        // each product of the backward pass reads one of the two; what neither needs is not kept alive
-        ctx->save_for_backward({gw ? x : Tensor(), gx ? weight : Tensor(), slope});
+        Tensor y = linear_run(x, weight, bias, (int)act, residual, keep ? &slope : nullptr);
+        // each product of the backward pass reads one of the two, the activation's derivative is kept or formed again from
+        // all three; what is not needed is not kept alive
+        const bool again = curved && !slope.defined();
+        ctx->save_for_backward({gw || again ? x : Tensor(), gx || again ? weight : Tensor(),
+                                again && bias.has_value() ? *bias : Tensor(), slope});
         ctx->saved_data["act"] = act;
         ctx->saved_data["k"] = weight.size(1);
         ctx->saved_data["n"] = weight.size(0);
@@ -158,7 +167,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     {
         refuse_double_backward("linear");
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &weight = saved[1], &slope = saved[2];
+        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &slope = saved[3];
         const Tensor& dy = grads[0];
         const int64_t act = ctx->saved_data["act"].toInt(), k = ctx->saved_data["k"].toInt(), n = ctx->saved_data["n"].toInt();
         const bool gx = ctx->needs_input_grad(0), gw = ctx->needs_input_grad(1);
@@ -170,14 +179,17 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         if (gx || gw || gb) {
             const Rows gr = rows_of(dy, n);
             Rows xr{}, wr{};
-            if (gw) xr = rows_of(x, k);
-            if (gx) wr = rows_of(weight, k);
+            if (x.defined()) xr = rows_of(x, k);
+            if (weight.defined()) wr = rows_of(weight, k);
+            Tensor b;
+            if (bias.defined()) b = vec(bias);
             if (gx) dx = torch::empty(with_last(dy, k), options.memory_format(torch::MemoryFormat::Contiguous));
             if (gw) dw = torch::empty({n, k}, options);
             if (gb) db = torch::empty({n}, options);
             Tensor ws = workspace_of(dy, api.linear_backward_ws(gr.rows, (int)k, (int)n, dtype, (int)act));
-            check(api.linear_backward(gr.rows, (int)k, (int)n, dtype, (int)act, gw ? xr.t.data_ptr() : nullptr, xr.stride,
-                                      gx ? wr.t.data_ptr() : nullptr, wr.stride, slope.defined() ? slope.data_ptr() : nullptr,
+            check(api.linear_backward(gr.rows, (int)k, (int)n, dtype, (int)act, x.defined() ? xr.t.data_ptr() : nullptr,
+                                      xr.stride, weight.defined() ? wr.t.data_ptr() : nullptr, wr.stride,
+                                      b.defined() ? b.data_ptr() : nullptr, slope.defined() ? slope.data_ptr() : nullptr,
                                       gr.t.data_ptr(), gr.stride, gx ? dx.data_ptr() : nullptr, gw ? dw.data_ptr() : nullptr,
                                       gb ? db.data_ptr() : nullptr, bytes_ptr(ws), stream_of(dy)));
         }
@@ -385,6 +397,7 @@ void ngs_decoder_bind(void* handle, const std::string& path)
     resolve(api.linear_forward_ws, handle, "ngs_linear_forward_workspace_bytes", path);
     resolve(api.linear_forward, handle, "ngs_linear_forward", path);
     resolve(api.linear_backward_ws, handle, "ngs_linear_backward_workspace_bytes", path);
+    resolve(api.linear_reads_slope, handle, "ngs_linear_backward_reads_slope", path);
     resolve(api.linear_backward, handle, "ngs_linear_backward", path);
     resolve(api.norm_forward, handle, "ngs_layer_norm_forward", path);
     resolve(api.norm_backward_ws, handle, "ngs_layer_norm_backward_workspace_bytes", path);

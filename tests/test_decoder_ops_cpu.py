@@ -27,7 +27,7 @@ def linear(lib, rows=4, k=8, n=3, dtype=0, act=0, x=SOME, ldx=8, w=SOME, ldw=8, 
 
 
 def linear_backward(lib, rows=4, k=8, n=3, dtype=0, act=0, x=SOME, w=SOME, slope=None, dy=SOME, lddy=3, dx=SOME, ws=SOME):
-    return lib.ngs_linear_backward(LL(rows), k, n, dtype, act, x, LL(8), w, LL(8), slope, dy, LL(lddy), dx, SOME, SOME, ws, None)
+    return lib.ngs_linear_backward(LL(rows), k, n, dtype, act, x, LL(8), w, LL(8), None, slope, dy, LL(lddy), dx, SOME, SOME, ws, None)
 
 
 def norm(lib, rows=4, d=8, dtype=0, wtype=0, eps=1e-5, x=SOME, ldx=8, y=SOME):

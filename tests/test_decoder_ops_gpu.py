@@ -57,7 +57,10 @@ def check_linear(ops, rows, k, n, dtype, act, bias, residual, train=True, first=
 LINEAR_SIZES = [(1, 1, 1), (1, 64, 128), (3, 39, 3), (5, 17, 31), (16, 8, 40), (33, 100, 65), (127, 128, 129),
                 (128, 64, 128), (130, 200, 300), (257, 513, 40), (1000, 39, 3), (300, 1030, 520), (4100, 24, 16),
                 (2, 4096, 1000), (64, 5000, 48), (7, 3, 700), (40, 2050, 33), (2600, 128, 128), (2049, 64, 96),
-                (515, 256, 256), (9, 1027, 2051), (12, 512, 512)]
+                (515, 256, 256), (9, 1027, 2051), (12, 512, 512),
+                # many narrow rows
+                (4096, 1, 1), (4097, 3, 5), (5000, 39, 3), (4999, 128, 128), (4100, 127, 129), (6001, 200, 24), (4200, 17, 100),
+                (4111, 256, 40), (9000, 64, 128), (4500, 8, 250), (5003, 65, 33), (4099, 33, 64), (70001, 40, 48)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -70,7 +73,8 @@ def test_linear_sizes(ops, size, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("act", ACTS)
-@pytest.mark.parametrize("size", [(70, 72, 40), (700, 39, 3), (3, 300, 260), (300, 64, 128)], ids=str)
+@pytest.mark.parametrize("size", [(70, 72, 40), (700, 39, 3), (3, 300, 260), (300, 64, 128), (4300, 39, 3),
+                                  (4301, 72, 40), (4302, 128, 128)], ids=str)
 def test_linear_activations(ops, size, act, dtype):
     """Every activation with and without bias and residual.  Small whole numbers give exact sums, so that relu's
     derivative at and next to zero is decided by the definition."""
@@ -81,7 +85,8 @@ def test_linear_activations(ops, size, act, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("case", [(300, 39, 3, 25, 64), (2500, 39, 64, 25, 64), (1, 39, 20, 25, 64), (140, 128, 130, 8, 144),
-                                  (300, 63, 64, 1, 65), (5, 256, 32, 0, 300)], ids=str)
+                                  (300, 63, 64, 1, 65), (5, 256, 32, 0, 300), (5000, 39, 64, 25, 64), (4500, 39, 3, 25, 64),
+                                  (4501, 128, 128, 0, 130), (4502, 63, 30, 1, 67)], ids=str)
 def test_linear_slices(ops, case, dtype):
     """Rows that are slices of wider ones (the 39 copied features of a feature row), aligned or not."""
     rows, k, n, first, pitch = case
@@ -137,7 +142,7 @@ def test_linear_zero_sizes(ops, size, dtype):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_linear_special_values(ops, dtype):
     """Infinities and NaN stay in their rows and columns, at every size of kernel."""
-    for rows, k, n in ((1, 100, 200), (6, 100, 200), (200, 39, 70), (300, 256, 256)):
+    for rows, k, n in ((1, 100, 200), (6, 100, 200), (200, 39, 70), (300, 256, 256), (5001, 39, 70), (4101, 128, 64)):
         g = gen(rows)
         x, w = normal(g, rows, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=0.1)
         clean = ops.linear(x, w)
@@ -162,8 +167,13 @@ def test_linear_special_values(ops, dtype):
 def test_linear_partial_gradients(ops):
     """Every subset of inputs that want gradients gets the gradients that all of them get."""
     g = gen(3)
-    tensors = [normal(g, 300, 40), normal(g, 24, 40, scale=0.2), normal(g, 24), normal(g, 300, 24)]
-    dy = normal(g, 300, 24)
+    for rows in (300, 5000):
+        partial_gradients(ops, g, rows)
+
+
+def partial_gradients(ops, g, rows):
+    tensors = [normal(g, rows, 40), normal(g, 24, 40, scale=0.2), normal(g, 24), normal(g, rows, 24)]
+    dy = normal(g, rows, 24)
 
     def run(subset, act):
         ts = [t.clone().requires_grad_(i in subset) for i, t in enumerate(tensors)]
