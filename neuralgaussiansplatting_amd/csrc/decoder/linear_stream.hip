@@ -189,7 +189,8 @@ __global__ __launch_bounds__(THREADS) void stream_forward_kernel(StreamForward<T
                 float z[N], y[N], slope[N];
 #pragma unroll
                 for (int e = 0; e < N; e++) z[e] = acc[u][e / 4][e % 4] + bias[col + e];
-                activate<N>(a.act, z, y, slope);
+                if (a.slope) activate<N>(a.act, z, y, slope);
+                else activate<N>(a.act, z, y, nullptr);
                 if (a.residual) {
                     float f[N];
                     unpack<T>(res[u], f);
@@ -429,15 +430,16 @@ template <typename T, int KS>
 static int stream_forward_launch(hipStream_t st, const StreamForward<T>& a)
 {
     const size_t lds = (size_t)a.lines * (KS * 64 + 4);
-    auto kernel = stream_forward_kernel<T, KS, 512>;
+    constexpr int THREADS = 256;
+    auto kernel = stream_forward_kernel<T, KS, THREADS>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return ngs_set_error("ngs_linear_forward", hipGetErrorString(e));
     }
-    const long long need = ((a.rows + 31) / 32 + 7) / 8;
+    const long long need = ((a.rows + 31) / 32 + THREADS / 64 - 1) / (THREADS / 64);
     const long long per_cu = (long long)(160 * 1024 / lds) < 4 ? (long long)(160 * 1024 / lds) : 4;
     const long long most = NGS_CUS * (per_cu > 0 ? per_cu : 1);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(need < most ? need : most)), dim3(512), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(need < most ? need : most)), dim3(THREADS), lds, st, a);
     return ngs_decoder_launched("ngs_linear_forward");
 }
 
