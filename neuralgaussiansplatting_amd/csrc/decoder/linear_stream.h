@@ -104,20 +104,32 @@ struct WeightTile {
     {
         return sizeof(T) == 2 ? (f >> 1) * 32 + (i >> 2) * 8 + (f & 1) * 4 + (i & 3) : f * 16 + i;
     }
+    // Results of two fragments of `across` (packed: two words of four columns each) as whole chunks: lane groups trade
+    // halves with their neighbours, after which group g holds the pair's chunk number chunk_of(g).  (Taking the columns in
+    // `column` order instead would make every read meet half its banks twice.)
+    static __device__ __forceinline__ int chunk_of(int g) { return sizeof(T) == 2 ? ((g & 1) << 1) | (g >> 1) : g; }
+    static __device__ __forceinline__ u32x4 join(u32x4 v)
+    {
+        if (sizeof(T) != 2) return v;
+        const auto lo = __builtin_amdgcn_permlane16_swap(v.x, v.z, false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap(v.y, v.w, false, false);
+        return (u32x4){lo[0], hi[0], lo[1], hi[1]};
+    }
     // fragment f of z's columns (the weight's rows), reduced along the weight's rows; chunks 4 s + g
     static __device__ __forceinline__ u32x4 along(const char* lds, int f, int s, int lane)
     {
         return *(const u32x4*)at(lds, column(f, lane & 15), s * 4 + (lane >> 4));
     }
-    // fragment f of dx's columns (the weight's columns), reduced across the weight's rows: those of chunks 4 s + g of dz
+    // fragment f of dx's columns (the weight's columns 16 f ...), reduced across the weight's rows: those of chunks
+    // 4 s + g of dz
     static __device__ __forceinline__ u32x4 across(const char* lds, int f, int s, int lane)
     {
         const int g = lane >> 4, i = lane & 15;
         if (sizeof(T) == 2) {
-            const int row = s * 32 + g * 8 + (i >> 2), c = (f >> 1) * 4 + (i & 3);
+            const int row = s * 32 + g * 8 + (i >> 2), c = f * 2 + ((i & 3) >> 1);
             typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at(lds, row, c) + (f & 1) * 8));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at(lds, row + 4, c) + (f & 1) * 8));
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at(lds, row, c) + (i & 1) * 8));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at(lds, row + 4, c) + (i & 1) * 8));
             const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
             return (u32x4){l.x, l.y, h.x, h.y};
         }
@@ -260,7 +272,9 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
 {
     constexpr int N = Chunk<T>::N, CK = KS * 4, CN = NS * 4, PARTS = N / 4;
     constexpr int TK = CK * N, TN = CN * N, TM = WAVES * 16;          // columns of x, columns of dz, rows of a tile
-    constexpr int FK = TK / 16, FN = TN / 16, EACH = (FK * FN + WAVES - 1) / WAVES;  // dW's fragments, and a wave's share
+    constexpr int FK = TK / 16, FN = TN / 16, EACH = (FK * FN + WAVES - 1) / WAVES;  // dW's fragments, and a wave's share:
+    constexpr int EK0 = EACH >= 8 ? 4 : EACH >= 2 ? 2 : 1, EK = EK0 < FK ? EK0 : FK, EN = EACH / EK;   // EK by EN of them
+    static_assert(FK % EK == 0 && FN % EN == 0, "shares fill dW");
     constexpr int STEPS = TM / (16 * PARTS);                          // reduction steps over a tile's rows
     typedef WeightTile<T, CK> W;
     typedef Tile<T, true, TK> TileX;
@@ -283,6 +297,7 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
     constexpr bool DB_MMA = sizeof(T) == 4;
     constexpr int DB_EACH = (FN + WAVES - 1) / WAVES;
     const bool tiles_wanted = a.dw || (DB_MMA && a.db);
+    const int kf0 = wave % (FK / EK) * EK, nf0 = wave / (FK / EK) * EN;  // this wave's share
     f32x4 acc[EACH], dbm[DB_EACH];
     float db[DB_MMA ? 1 : NS][N];
 #pragma unroll
@@ -300,7 +315,7 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
         const long long r = t * TM + wave * 16 + i;
         if (r >= a.rows) return;
 #pragma unroll
-        for (int b = 0; b < KS; b++) RowChunks<T>::store(a.dx + r * a.k, dx[b], b * 4 + g, b * 4, a.k);
+        for (int b = 0; b < KS; b++) RowChunks<T>::store(a.dx + r * a.k, dx[b], b * 4 + W::chunk_of(g), b * 4, a.k);
     };
     auto fetch = [&](long long t) {
         const long long r = t * TM + wave * 16 + i, row = r < a.rows ? r : a.rows - 1;
@@ -371,8 +386,8 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
                 float d[N];
 #pragma unroll
                 for (int e = 0; e < N; e++) d[e] = c[e / 4][e % 4];
-                dx[b] = pack<T>(d);
-                if (!HOLD && there) RowChunks<T>::store(a.dx + (t * TM + wave * 16 + i) * a.k, dx[b], b * 4 + g, b * 4, a.k);
+                dx[b] = W::join(pack<T>(d));
+                if (!HOLD && there) RowChunks<T>::store(a.dx + (t * TM + wave * 16 + i) * a.k, dx[b], b * 4 + W::chunk_of(g), b * 4, a.k);
             }
         }
         if (tiles_wanted) {
@@ -387,12 +402,14 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
                         if (f < FN) dbm[e] = mma(ones, TileZ::fragment(tile_z, f, s, lane), dbm[e], (const T*)nullptr);
                     }
                 }
+                if (nf0 < FN) {
+                    u32x4 f[EK], h[EN];
 #pragma unroll
-                for (int e = 0; e < EACH; e++) {
-                    const int f = wave * EACH + e;
-                    if (FK * FN % WAVES != 0 && f >= FK * FN) break;
-                    acc[e] = mma(TileX::fragment(tile_x, f % FK, s, lane), TileZ::fragment(tile_z, f / FK, s, lane), acc[e],
-                                 (const T*)nullptr);
+                    for (int e = 0; e < EK; e++) f[e] = TileX::fragment(tile_x, kf0 + e, s, lane);
+#pragma unroll
+                    for (int e = 0; e < EN; e++) h[e] = TileZ::fragment(tile_z, nf0 + e, s, lane);
+#pragma unroll
+                    for (int e = 0; e < EACH; e++) acc[e] = mma(f[e % EK], h[e / EK], acc[e], (const T*)nullptr);
                 }
             }
             __syncthreads();
@@ -404,8 +421,8 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
     if (a.dw) {
 #pragma unroll
         for (int e = 0; e < EACH; e++) {
-            const int f = wave * EACH + e, col = (f % FK) * 16 + g * 4, row = (f / FK) * 16 + i;
-            if (f < FK * FN && row < a.n && col < a.k) {
+            const int col = (kf0 + e % EK) * 16 + g * 4, row = (nf0 + e / EK) * 16 + i;
+            if (nf0 < FN && row < a.n && col < a.k) {
                 const float v[4] = {acc[e][0], acc[e][1], acc[e][2], acc[e][3]};
                 store4(out + (long long)row * a.k + col, v, a.k - col);
             }
