@@ -19,11 +19,59 @@ struct Product {
     long long ldp, ldq;  // elements between neighbouring rows of the array as it lies in memory
     int np;
     long long nq, nr;
+    long long width_p, width_q;  // rows of P and Q as far as they may be read: np and nq, or more where they are padded
     long long tiles_p, tiles_q;
     int splits;          // the reduction is cut into this many runs of `run` elements (a multiple of a step's)
     long long run;
     Epilogue<T> epi;
 };
+
+// Which tile and which run of the reduction a workgroup computes.  Workgroups go to the dies in turn: each die takes a
+// contiguous run of tiles, whose operands meet in its cache.
+struct Place {
+    long long p0, q0, split, r_begin, r_end;
+    bool there;
+};
+template <typename T, int TP, int TQ>
+__device__ __forceinline__ Place place_of(const Product<T>& a)
+{
+    const long long tiles = a.tiles_p * a.tiles_q, groups = tiles * a.splits;
+    const long long per = (groups + NGS_XCDS - 1) / NGS_XCDS;
+    const long long t = (long long)(blockIdx.x % NGS_XCDS) * per + blockIdx.x / NGS_XCDS;
+    Place w;
+    w.there = t < groups;
+    w.split = t / tiles;
+    const long long tile = t - w.split * tiles;
+    w.p0 = (tile % a.tiles_p) * TP;
+    w.q0 = (tile / a.tiles_p) * TQ;
+    w.r_begin = w.split * a.run;
+    w.r_end = w.r_begin + a.run < a.nr ? w.r_begin + a.run : a.nr;
+    return w;
+}
+
+// A wave's MP x MQ fragments from (p0, q0) on: a lane holds four neighbouring p of one q.
+template <typename T, int MP, int MQ>
+__device__ __forceinline__ void finish_tile(const Product<T>& a, const f32x4 (&acc)[MP][MQ], long long p0, long long q0,
+                                            long long split, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < MP; i++) {
+        const int p = (int)p0 + i * 16 + (lane >> 4) * 4;
+        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p < a.np && a.epi.bias && !a.epi.partial) load4(a.epi.bias + p, bias, a.np - p);
+#pragma unroll
+        for (int j = 0; j < MQ; j++) {
+            const long long q = q0 + j * 16 + (lane & 15);
+            if (p >= a.np || q >= a.nq) continue;
+            if (a.epi.partial) {
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                store4(a.epi.partial + (split * a.nq + q) * a.np + p, v, a.np - p);
+            } else {
+                finish4(a.epi, q, p, acc[i][j], bias);
+            }
+        }
+    }
+}
 
 // A workgroup of WP x WQ waves computes a TP x TQ tile of one run of the reduction; each step's operands travel
 // through registers into shared memory while the step before is multiplied.
@@ -40,14 +88,9 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_kernel(Product<T> a)
     __shared__ __attribute__((aligned(16))) char sq[TQ * ROW_BYTES];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP, wq = wave / WP;
-    // workgroups go to the dies in turn: each die takes a contiguous run of tiles, whose operands meet in its cache
-    const long long tiles = a.tiles_p * a.tiles_q, groups = tiles * a.splits;
-    const long long per = (groups + NGS_XCDS - 1) / NGS_XCDS;
-    const long long t = (long long)(blockIdx.x % NGS_XCDS) * per + blockIdx.x / NGS_XCDS;
-    if (t >= groups) return;
-    const long long split = t / tiles, tile = t - split * tiles;
-    const long long p0 = (tile % a.tiles_p) * TP, q0 = (tile / a.tiles_p) * TQ;
-    const long long r_begin = split * a.run, r_end = r_begin + a.run < a.nr ? r_begin + a.run : a.nr;
+    const Place at = place_of<T, TP, TQ>(a);
+    if (!at.there) return;
+    const long long p0 = at.p0, q0 = at.q0, r_begin = at.r_begin, r_end = at.r_end, split = at.split;
 
     f32x4 acc[MP][MQ];
 #pragma unroll
@@ -85,24 +128,193 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_kernel(Product<T> a)
         }
     }
 
-    // a lane holds four neighbouring p of one q
+    finish_tile<T, MP, MQ>(a, acc, p0 + wp * MP * 16, q0 + wq * MQ * 16, split, lane);
+}
+
+// The same with operands that lie on 16-byte boundaries: they go from memory into shared memory without passing
+// through registers, the next step's while this one is multiplied.  With 256 x 256 tiles and eight waves (128 x 64 each)
+// the matrix units have 2048 cycles of work per step of 64 16-bit elements and the fragments' reads take 1536 of the
+// shared memory's.
+//
+// A wave's load fills 1 KiB of a tile in lane order; which chunk a lane fetches undoes the exchange of the tile's layout.
+// What lies beyond the operand's end reads as zero (the resource's bound), and so does, along, what lies beyond the
+// reduction's (an offset past the bound).
+template <typename T, bool ACROSS, int ROWS, int WAVES>
+struct TileLoader {
+    static constexpr int N = Chunk<T>::N, STEP = ROW_BYTES / (int)sizeof(T), LINE = ROWS * (int)sizeof(T) / 16;
+    static constexpr int LOADS = ROWS * ROW_BYTES / 1024 / WAVES;
+    static_assert(LOADS * WAVES * 1024 == ROWS * ROW_BYTES, "loads divide over the waves");
+    uint32_t offset[LOADS];
+    const char* base;
+    long long left, advance;  // bytes from base to the operand's end (of the reduction, across), and per step
+    int first;                // along: this lane's first reduction element in a step
+
+    __device__ __forceinline__ TileLoader(const T* p, long long ld, long long row0, long long rows, long long r0, long long r_end,
+                                          int wave, int lane)
+    {
+        if (!ACROSS) {
+            base = (const char*)(p + row0 * ld + r0);
+            left = ((rows - 1 - row0) * ld + (r_end - r0)) * (long long)sizeof(T);
+            advance = ROW_BYTES;
+            const int c = (lane & 7) ^ (lane >> 3);
+            first = c * N;
 #pragma unroll
-    for (int i = 0; i < MP; i++) {
-        const int p = (int)p0 + (wp * MP + i) * 16 + (lane >> 4) * 4;
-        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (p < a.np && a.epi.bias && !a.epi.partial) load4(a.epi.bias + p, bias, a.np - p);
+            for (int k = 0; k < LOADS; k++)
+                offset[k] = (uint32_t)((k * WAVES + wave) * 8 + (lane >> 3)) * (uint32_t)(ld * sizeof(T)) + c * 16;
+        } else {
+            base = (const char*)(p + r0 * ld + row0);
+            left = ((r_end - 1 - r0) * ld + (rows - row0)) * (long long)sizeof(T);
+            advance = STEP * ld * (long long)sizeof(T);
+            first = 0;
 #pragma unroll
-        for (int j = 0; j < MQ; j++) {
-            const long long q = q0 + (wq * MQ + j) * 16 + (lane & 15);
-            if (p >= a.np || q >= a.nq) continue;
-            if (a.epi.partial) {
-                float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                store4(a.epi.partial + (split * a.nq + q) * a.np + p, v, a.np - p);
-            } else {
-                finish4(a.epi, q, p, acc[i][j], bias);
+            for (int k = 0; k < LOADS; k++) {
+                const int i = (k * WAVES + wave) * 64 + lane, line = i / LINE;
+                const int c = (i % LINE) ^ (Tile<T, true, ROWS>::segment_swap(line) * Tile<T, true, ROWS>::SEG);
+                offset[k] = (uint32_t)line * (uint32_t)(ld * sizeof(T)) + c * 16;
             }
         }
     }
+    // the next step's tile into `lds` (an address in shared memory); `length`: reduction elements that are left
+    __device__ __forceinline__ void load(uint32_t lds, long long length, int wave)
+    {
+        const uint64_t b = (uint64_t)base;
+        const long long bytes = left < 0 ? 0 : left < 0x7ffffff0 ? left : 0x7ffffff0;
+        u32x4 rsrc;
+        rsrc.x = __builtin_amdgcn_readfirstlane((uint32_t)b);
+        rsrc.y = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32) & 0xffffu);
+        rsrc.z = __builtin_amdgcn_readfirstlane((uint32_t)bytes);
+        rsrc.w = 0x00020000u;
+        const bool beyond = !ACROSS && first >= length;
+#pragma unroll
+        for (int k = 0; k < LOADS; k++) {
+            const uint32_t o = beyond ? 0x7ffffff0u : offset[k];
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (k * WAVES + wave) * 1024);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :: "s"(to), "v"(o), "s"(rsrc) : "memory");
+        }
+        base += advance;
+        left -= advance;
+    }
+};
+
+// A wave's results through its own piece of shared memory, 16 rows at a time, so that they leave as whole lines and the
+// epilogue's code is there once per 16 rows rather than once per fragment.  BARE: no epilogue.
+template <typename T, int MP, int MQ, bool BARE>
+__device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&acc)[MP][MQ], float* lds, long long p0,
+                                            long long q0, long long split, int lane)
+{
+    constexpr int N = Chunk<T>::N, PITCH = MP * 16 + 4, LANES = MP * 16 / N, ROWS = 64 / LANES;
+    const int g = lane >> 4, i = lane & 15;
+    if (a.epi.partial) {
+#pragma unroll
+        for (int f = 0; f < MP; f++) {
+            const int p = (int)p0 + f * 16 + g * 4;
+#pragma unroll
+            for (int j = 0; j < MQ; j++) {
+                const long long q = q0 + j * 16 + i;
+                const float v[4] = {acc[f][j][0], acc[f][j][1], acc[f][j][2], acc[f][j][3]};
+                if (p < a.np && q < a.nq) store4(a.epi.partial + (split * a.nq + q) * a.np + p, v, a.np - p);
+            }
+        }
+        return;
+    }
+    const int col = (lane % LANES) * N, p = (int)p0 + col, valid = a.np - p;
+    float bias[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) bias[e] = 0.0f;
+    if (!BARE && a.epi.bias && valid > 0) unpack<T>(load16_head(a.epi.bias + p, valid), bias);
+#pragma unroll
+    for (int j = 0; j < MQ; j++) {
+#pragma unroll
+        for (int f = 0; f < MP; f++) *(f32x4*)&lds[i * PITCH + f * 16 + g * 4] = acc[f][j];
+        __builtin_amdgcn_wave_barrier();  // (one wave's accesses to shared memory are in order)
+#pragma unroll 1
+        for (int r = lane / LANES; r < 16; r += ROWS) {
+            const long long q = q0 + j * 16 + r;
+            if (q >= a.nq || valid <= 0) continue;
+            float z[N], y[N];
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const f32x4 v = *(const f32x4*)&lds[r * PITCH + col + e];
+#pragma unroll
+                for (int k = 0; k < 4; k++) z[e + k] = v[k] + bias[e + k];
+            }
+            if constexpr (BARE) {
+                store16_head(a.epi.y + q * a.np + p, pack<T>(z), valid);
+            } else {
+                float slope[N], res[N];
+                if (a.epi.residual) unpack<T>(load16_head(a.epi.residual + q * a.epi.ldr + p, valid), res);
+                activate<N>(a.epi.act, z, y, slope);
+                if (a.epi.residual) {
+#pragma unroll
+                    for (int e = 0; e < N; e++) y[e] += res[e];
+                }
+                store16_head(a.epi.y + q * a.np + p, pack<T>(y), valid);
+                if (a.epi.slope) {
+                    typedef typename Slope<T>::type S;
+                    static_assert(sizeof(S) == sizeof(T), "a chunk of derivatives beside a chunk of results");
+                    store16_head(a.epi.slope + q * a.np + p, pack<S>(slope), valid);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <typename T, bool P_ACROSS, bool Q_ACROSS, int TP, int TQ, int WP, int WQ>
+__global__ __launch_bounds__(64 * WP * WQ) void product_direct_kernel(Product<T> a)
+{
+    typedef Tile<T, P_ACROSS, TP> TileP;
+    typedef Tile<T, Q_ACROSS, TQ> TileQ;
+    constexpr int WAVES = WP * WQ, STEP = TileP::STEP, MP = TP / WP / 16, MQ = TQ / WQ / 16;
+    constexpr int P_BYTES = TP * ROW_BYTES, STAGE = (TP + TQ) * ROW_BYTES;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave % WP, wq = wave / WP;
+    const Place at = place_of<T, TP, TQ>(a);
+    if (!at.there) return;
+
+    f32x4 acc[MP][MQ];
+#pragma unroll
+    for (int i = 0; i < MP; i++)
+#pragma unroll
+        for (int j = 0; j < MQ; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+
+    TileLoader<T, P_ACROSS, TP, WAVES> lp(a.p, a.ldp, at.p0, a.width_p, at.r_begin, at.r_end, wave, lane);
+    TileLoader<T, Q_ACROSS, TQ, WAVES> lq(a.q, a.ldq, at.q0, a.width_q, at.r_begin, at.r_end, wave, lane);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    const long long length = at.r_end - at.r_begin;
+    if (length > 0) {
+        lp.load(lds0, length, wave);
+        lq.load(lds0 + P_BYTES, length, wave);
+    }
+    int buf = 0;
+    for (long long r = 0; r < length; r += STEP) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // this step's tiles are there, the other buffer is free
+        if (r + STEP < length) {
+            const uint32_t to = lds0 + (buf ^ 1) * STAGE;
+            lp.load(to, length - r - STEP, wave);
+            lq.load(to + P_BYTES, length - r - STEP, wave);
+        }
+        const char *const sp = lds + buf * STAGE, *const sq = sp + P_BYTES;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            u32x4 f[MP], h[MQ];
+#pragma unroll
+            for (int j = 0; j < MQ; j++) h[j] = TileQ::fragment(sq, wq * MQ + j, s, lane);
+#pragma unroll
+            for (int i = 0; i < MP; i++) f[i] = TileP::fragment(sp, wp * MP + i, s, lane);
+#pragma unroll
+            for (int i = 0; i < MP; i++)
+#pragma unroll
+                for (int j = 0; j < MQ; j++) acc[i][j] = mma(f[i], h[j], acc[i][j], (const T*)nullptr);
+        }
+        buf ^= 1;
+    }
+    __syncthreads();  // the tiles are done with
+    static_assert(WAVES * 16 * (MP * 16 + 4) * 4 <= 2 * STAGE, "a piece of the tiles' memory for each wave");
+    finish_wide<T, MP, MQ, P_ACROSS>(a, acc, (float*)lds + wave * 16 * (MP * 16 + 4), at.p0 + wp * MP * 16, at.q0 + wq * MQ * 16,
+                                     at.split, lane);
 }
 
 // Adds up the runs of a product that was cut along its reduction, in their order, and finishes it.
@@ -226,19 +438,21 @@ struct Shape {
     size_t partial_bytes(long long np, long long nq) const { return splits > 1 ? (size_t)splits * np * nq * 4 : 0; }
 };
 
-// Tiles are 128 wide unless the matrix is 32 or narrower; a reduction is cut until the tiles and its runs fill the
-// chip twice, each run at least four steps long.
-static Shape product_shape(long long np, long long nq, long long nr, int dtype)
+// Through registers, tiles are 128 wide unless the matrix is 32 or narrower; a reduction is cut until the tiles and its
+// runs fill the chip twice, each run at least four steps long.
+// Directly (16-bit types), tiles are 256 x 256 where those fill the chip, 128 x 128 otherwise.
+static Shape product_shape(long long np, long long nq, long long nr, int dtype, bool direct)
 {
     Shape s;
     s.tp = np <= 32 ? 32 : 128;
     s.tq = nq <= 32 ? 32 : 128;
+    if (direct && ((np + 255) / 256) * ((nq + 255) / 256) >= NGS_CUS / 2) s.tp = s.tq = 256;
     s.tiles_p = (np + s.tp - 1) / s.tp;
     s.tiles_q = (nq + s.tq - 1) / s.tq;
     const long long step = ROW_BYTES / (long long)ngs_decoder_size(dtype), steps = (nr + step - 1) / step;
     const long long tiles = s.tiles_p * s.tiles_q;
     long long cut = 1;
-    if (tiles > 0 && tiles < NGS_CUS) {
+    if (tiles > 0 && tiles < NGS_CUS && s.tp < 256) {
         cut = (2 * NGS_CUS + tiles - 1) / tiles;
         if (cut > steps / 4) cut = steps / 4;
         if (cut < 1) cut = 1;
@@ -249,9 +463,34 @@ static Shape product_shape(long long np, long long nq, long long nr, int dtype)
     return s;
 }
 
-template <typename T, bool PA, bool QA>
-static int launch_product(hipStream_t st, const Shape& s, Product<T> a, float* partial)
+// Whether product_direct_kernel has a tile for these sizes
+static bool direct_sizes(long long np, long long nq, int dtype) { return dtype != NGS_FLOAT32 && np > 32 && nq > 32; }
+
+// Whether it can read an operand: whole aligned chunks, and offsets within a tile's rows in 31 bits
+template <typename T>
+static bool direct_operand(const T* p, long long ld, bool across, long long width, long long nr)
 {
+    const long long n = Chunk<T>::N;
+    return (uintptr_t)p % 16 == 0 && ld % n == 0 && (across ? width : nr) % n == 0 && ld >= (across ? width : nr) &&
+           ld < (1LL << 21);
+}
+
+static size_t partial_bytes(long long np, long long nq, long long nr, int dtype)
+{
+    const size_t a = product_shape(np, nq, nr, dtype, false).partial_bytes(np, nq);
+    if (!direct_sizes(np, nq, dtype)) return a;
+    const size_t b = product_shape(np, nq, nr, dtype, true).partial_bytes(np, nq);
+    return a > b ? a : b;
+}
+
+template <typename T, bool PA, bool QA>
+static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partial)
+{
+    bool direct = false;
+    if constexpr (sizeof(T) == 2)
+        direct = direct_sizes(a.np, a.nq, dtype) && direct_operand(a.p, a.ldp, PA, a.width_p, a.nr) &&
+                 direct_operand(a.q, a.ldq, QA, a.width_q, a.nr);
+    const Shape s = product_shape(a.np, a.nq, a.nr, dtype, direct);
     a.tiles_p = s.tiles_p;
     a.tiles_q = s.tiles_q;
     a.splits = s.splits;
@@ -260,14 +499,22 @@ static int launch_product(hipStream_t st, const Shape& s, Product<T> a, float* p
     a.epi.partial = s.splits > 1 ? partial : nullptr;
     if (s.groups() > 0x7fffffffLL) return ngs_set_error("ngs_linear", "too many rows");
     const dim3 grid((unsigned)s.groups());
-    if (s.tp == 128 && s.tq == 128)
+    if constexpr (sizeof(T) == 2) {
+        if (direct && s.tp == 256)
+            hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 256, 256, 2, 4>), grid, dim3(512), 0, st, a);
+        else if (direct)
+            hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
+    }
+    if (direct) {
+    } else if (s.tp == 128 && s.tq == 128) {
         hipLaunchKernelGGL((product_kernel<T, PA, QA, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
-    else if (s.tp == 128)
+    } else if (s.tp == 128) {
         hipLaunchKernelGGL((product_kernel<T, PA, QA, 128, 32, 4, 1>), grid, dim3(256), 0, st, a);
-    else if (s.tq == 128)
+    } else if (s.tq == 128) {
         hipLaunchKernelGGL((product_kernel<T, PA, QA, 32, 128, 1, 4>), grid, dim3(256), 0, st, a);
-    else
+    } else {
         hipLaunchKernelGGL((product_kernel<T, PA, QA, 32, 32, 2, 2>), grid, dim3(256), 0, st, a);
+    }
     if (s.splits > 1) {
         Epilogue<T> e = a.epi;
         const long long items = (a.np + 3LL) / 4 * a.nq;
@@ -282,7 +529,6 @@ static inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // Backward workspace: dz (when there is an activation), the column sums' partials, the cut products' partials (the
 // two products run one after the other and share them).
 struct BackwardPlan {
-    Shape dx, dw;
     int across;
     long long col_blocks, row_blocks;
     size_t sums_at, partial_at, total;
@@ -292,8 +538,6 @@ static BackwardPlan backward_plan(long long rows, int k, int n, int dtype, int a
 {
     BackwardPlan b;
     const long long size = (long long)ngs_decoder_size(dtype), chunk = 16 / size;
-    b.dx = product_shape(k, rows, n, dtype);
-    b.dw = product_shape(k, n, rows, dtype);
     const long long chunks = (n + chunk - 1) / chunk;
     b.across = 1;
     while (b.across < 64 && b.across < chunks) b.across *= 2;
@@ -304,7 +548,7 @@ static BackwardPlan backward_plan(long long rows, int k, int n, int dtype, int a
     if (b.row_blocks < 1) b.row_blocks = 1;
     b.sums_at = act == NGS_ACT_NONE ? 0 : align256((size_t)rows * n * size);
     b.partial_at = b.sums_at + align256((size_t)b.row_blocks * n * 4);
-    const size_t p1 = b.dx.partial_bytes(k, rows), p2 = b.dw.partial_bytes(k, n);
+    const size_t p1 = partial_bytes(k, rows, n, dtype), p2 = partial_bytes(k, n, rows, dtype);
     b.total = b.partial_at + align256(p1 > p2 ? p1 : p2) + 256;
     return b;
 }
@@ -331,7 +575,9 @@ static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtyp
     a.epi.np = n;
     if (ngs_stream_forward_takes(rows, k, n, dtype))
         return ngs_stream_forward<T>(st, rows, k, n, dtype, a.q, ldx, a.p, ldw, a.epi);
-    return launch_product<T, false, false>(st, product_shape(n, rows, k, dtype), a, (float*)workspace);
+    a.width_p = n;
+    a.width_q = rows;
+    return launch_product<T, false, false>(st, dtype, a, (float*)workspace);
 }
 
 template <typename T>
@@ -369,8 +615,10 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
         a.np = k;
         a.nq = rows;
         a.nr = n;
+        a.width_p = k;
+        a.width_q = rows;
         a.epi.y = (T*)dx;
-        if (launch_product<T, true, false>(st, b.dx, a, partial)) return 1;
+        if (launch_product<T, true, false>(st, dtype, a, partial)) return 1;
     }
     if (dw) {
         Product<T> a = {};
@@ -381,8 +629,10 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
         a.np = k;
         a.nq = n;
         a.nr = rows;
+        a.width_p = k;
+        a.width_q = n;
         a.epi.y = (T*)dw;
-        if (launch_product<T, true, true>(st, b.dw, a, partial)) return 1;
+        if (launch_product<T, true, true>(st, dtype, a, partial)) return 1;
     }
     return 0;
 }
@@ -403,7 +653,7 @@ extern "C" size_t ngs_linear_forward_workspace_bytes(long long rows, int in_feat
 {
     if (rows <= 0 || out_features <= 0 || in_features < 0 || rows > (1LL << 40) || !ngs_decoder_dtype(dtype)) return 0;
     if (ngs_stream_forward_takes(rows, in_features, out_features, dtype)) return 0;
-    return product_shape(out_features, rows, in_features, dtype).partial_bytes(out_features, rows);
+    return partial_bytes(out_features, rows, in_features, dtype);
 }
 
 extern "C" int ngs_linear_forward(long long rows, int in_features, int out_features, int dtype, int activation,
