@@ -19,7 +19,9 @@ struct Product {
     long long ldp, ldq;  // elements between neighbouring rows of the array as it lies in memory
     int np;
     long long nq, nr;
-    long long width_p, width_q;  // rows of P and Q as far as they may be read: np and nq, or more where they are padded
+    // how far rows may be read (zeros behind their end where they are padded): of an operand that lies across, its np or
+    // nq columns; of one that lies along, the reduction's nr
+    long long width_p, width_q, along;
     long long tiles_p, tiles_q;
     int splits;          // the reduction is cut into this many runs of `run` elements (a multiple of a step's)
     long long run;
@@ -199,11 +201,14 @@ struct TileLoader {
 
 // A wave's results through its own piece of shared memory, 16 rows at a time, so that they leave as whole lines and the
 // epilogue's code is there once per 16 rows rather than once per fragment.  BARE: no epilogue.
+template <int MP>
+constexpr int finish_wide_bytes() { return 16 * (MP * 16 + 4) * 4 + 16 * MP * 16 * 2; }  // a wave's piece
+
 template <typename T, int MP, int MQ, bool BARE>
 __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&acc)[MP][MQ], float* lds, long long p0,
                                             long long q0, long long split, int lane)
 {
-    constexpr int N = Chunk<T>::N, PITCH = MP * 16 + 4, LANES = MP * 16 / N, ROWS = 64 / LANES;
+    constexpr int N = Chunk<T>::N, PITCH = MP * 16 + 4, LANES = MP * 16 / N, ROWS = 64 / LANES, TRIPS = 16 / ROWS;
     const int g = lane >> 4, i = lane & 15;
     if (a.epi.partial) {
 #pragma unroll
@@ -223,13 +228,31 @@ __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&a
 #pragma unroll
     for (int e = 0; e < N; e++) bias[e] = 0.0f;
     if (!BARE && a.epi.bias && valid > 0) unpack<T>(load16_head(a.epi.bias + p, valid), bias);
+    // the residual's chunks of the next 16 rows are on their way while these are finished; they wait in shared memory, so
+    // that the loop over the rows can stay a loop
+    u32x4 res[TRIPS];
+    u32x4* const parked = (u32x4*)(lds + 16 * PITCH) + lane;
+    auto fetch = [&](int j) {
+#pragma unroll
+        for (int t = 0; t < TRIPS; t++) {
+            const long long q = q0 + j * 16 + t * ROWS + lane / LANES;
+            res[t] = load16_head(a.epi.residual + (q < a.nq ? q : 0) * a.epi.ldr + p, valid);
+        }
+    };
+    if (!BARE && a.epi.residual) fetch(0);
 #pragma unroll
     for (int j = 0; j < MQ; j++) {
 #pragma unroll
         for (int f = 0; f < MP; f++) *(f32x4*)&lds[i * PITCH + f * 16 + g * 4] = acc[f][j];
+        if (!BARE && a.epi.residual) {
+#pragma unroll
+            for (int t = 0; t < TRIPS; t++) parked[t * 64] = res[t];
+            if (j + 1 < MQ) fetch(j + 1);
+        }
         __builtin_amdgcn_wave_barrier();  // (one wave's accesses to shared memory are in order)
 #pragma unroll 1
-        for (int r = lane / LANES; r < 16; r += ROWS) {
+        for (int t = 0; t < TRIPS; t++) {
+            const int r = t * ROWS + lane / LANES;
             const long long q = q0 + j * 16 + r;
             if (q >= a.nq || valid <= 0) continue;
             float z[N], y[N];
@@ -242,19 +265,22 @@ __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&a
             if constexpr (BARE) {
                 store16_head(a.epi.y + q * a.np + p, pack<T>(z), valid);
             } else {
-                float slope[N], res[N];
-                if (a.epi.residual) unpack<T>(load16_head(a.epi.residual + q * a.epi.ldr + p, valid), res);
-                activate<N>(a.epi.act, z, y, slope);
-                if (a.epi.residual) {
-#pragma unroll
-                    for (int e = 0; e < N; e++) y[e] += res[e];
-                }
-                store16_head(a.epi.y + q * a.np + p, pack<T>(y), valid);
+                float slope[N];
                 if (a.epi.slope) {
                     typedef typename Slope<T>::type S;
                     static_assert(sizeof(S) == sizeof(T), "a chunk of derivatives beside a chunk of results");
+                    activate<N>(a.epi.act, z, y, slope);
                     store16_head(a.epi.slope + q * a.np + p, pack<S>(slope), valid);
+                } else {
+                    activate<N>(a.epi.act, z, y, nullptr);
                 }
+                if (a.epi.residual) {
+                    float f[N];
+                    unpack<T>(parked[t * 64], f);
+#pragma unroll
+                    for (int e = 0; e < N; e++) y[e] += f[e];
+                }
+                store16_head(a.epi.y + q * a.np + p, pack<T>(y), valid);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -279,8 +305,9 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_direct_kernel(Product<T>
 #pragma unroll
         for (int j = 0; j < MQ; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
-    TileLoader<T, P_ACROSS, TP, WAVES> lp(a.p, a.ldp, at.p0, a.width_p, at.r_begin, at.r_end, wave, lane);
-    TileLoader<T, Q_ACROSS, TQ, WAVES> lq(a.q, a.ldq, at.q0, a.width_q, at.r_begin, at.r_end, wave, lane);
+    const long long r_read = at.r_end == a.nr ? a.along : at.r_end;
+    TileLoader<T, P_ACROSS, TP, WAVES> lp(a.p, a.ldp, at.p0, a.width_p, at.r_begin, P_ACROSS ? at.r_end : r_read, wave, lane);
+    TileLoader<T, Q_ACROSS, TQ, WAVES> lq(a.q, a.ldq, at.q0, a.width_q, at.r_begin, Q_ACROSS ? at.r_end : r_read, wave, lane);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     const long long length = at.r_end - at.r_begin;
     if (length > 0) {
@@ -312,8 +339,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_direct_kernel(Product<T>
         buf ^= 1;
     }
     __syncthreads();  // the tiles are done with
-    static_assert(WAVES * 16 * (MP * 16 + 4) * 4 <= 2 * STAGE, "a piece of the tiles' memory for each wave");
-    finish_wide<T, MP, MQ, P_ACROSS>(a, acc, (float*)lds + wave * 16 * (MP * 16 + 4), at.p0 + wp * MP * 16, at.q0 + wq * MQ * 16,
+    static_assert(WAVES * finish_wide_bytes<MP>() <= 2 * STAGE, "a piece of the tiles' memory for each wave");
+    finish_wide<T, MP, MQ, P_ACROSS>(a, acc, (float*)(lds + wave * finish_wide_bytes<MP>()), at.p0 + wp * MP * 16, at.q0 + wq * MQ * 16,
                                      at.split, lane);
 }
 
@@ -347,7 +374,7 @@ __global__ __launch_bounds__(256) void product_finish_kernel(const float* __rest
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(long long rows, int n, int across, const T* __restrict__ dy,
                                                         long long lddy, const typename Slope<T>::type* __restrict__ slope,
-                                                        T* __restrict__ dz, float* __restrict__ partial)
+                                                        T* __restrict__ dz, long long lddz, float* __restrict__ partial)
 {
     constexpr int N = Chunk<T>::N;
     __shared__ float sums[256 * N];
@@ -371,8 +398,8 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long rows, int n, i
                     for (int i = 0; i < N; i++)
                         if (i < valid) g[i] *= (float)slope[r * n + col + i];
                 }
-                if (dz) store16_head(dz + r * n + col, pack<T>(g), valid);
             }
+            if (dz) store16_head(dz + r * lddz + col, pack<T>(g), lddz - col);
 #pragma unroll
             for (int i = 0; i < N; i++) acc[i] += g[i];
         }
@@ -438,15 +465,25 @@ struct Shape {
     size_t partial_bytes(long long np, long long nq) const { return splits > 1 ? (size_t)splits * np * nq * 4 : 0; }
 };
 
+static inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
 // Through registers, tiles are 128 wide unless the matrix is 32 or narrower; a reduction is cut until the tiles and its
 // runs fill the chip twice, each run at least four steps long.
-// Directly (16-bit types), tiles are 256 x 256 where those fill the chip, 128 x 128 otherwise.
+// Directly (16-bit types), tiles are 256 x 256, one to a compute unit, or 128 x 128, two at a time.  A round of the
+// former takes one and a half times as long as one of the latter (8192 x 4096 -> 4096 bfloat16: 2 rounds 233 us, 4 rounds
+// 317 us; 6144 x 1024 -> 3200: 2 rounds 64 us, 2.3 rounds 51 us; 4096 x 1024 -> 2048: 35 us and 24 us, one round each); a
+// last round of small tiles that does not fill the chip costs about 0.6 of a full one.
 static Shape product_shape(long long np, long long nq, long long nr, int dtype, bool direct)
 {
     Shape s;
     s.tp = np <= 32 ? 32 : 128;
     s.tq = nq <= 32 ? 32 : 128;
-    if (direct && ((np + 255) / 256) * ((nq + 255) / 256) >= NGS_CUS / 2) s.tp = s.tq = 256;
+    if (direct) {
+        const long long large = ((np + 255) / 256) * ((nq + 255) / 256), small = ((np + 127) / 128) * ((nq + 127) / 128);
+        const double large_cost = 1.5 * (double)((large + NGS_CUS - 1) / NGS_CUS);
+        const double small_cost = (double)(small / (2 * NGS_CUS)) + (small % (2 * NGS_CUS) ? 0.6 : 0.0);
+        if (large_cost < small_cost) s.tp = s.tq = 256;
+    }
     s.tiles_p = (np + s.tp - 1) / s.tp;
     s.tiles_q = (nq + s.tq - 1) / s.tq;
     const long long step = ROW_BYTES / (long long)ngs_decoder_size(dtype), steps = (nr + step - 1) / step;
@@ -468,11 +505,42 @@ static bool direct_sizes(long long np, long long nq, int dtype) { return dtype !
 
 // Whether it can read an operand: whole aligned chunks, and offsets within a tile's rows in 31 bits
 template <typename T>
-static bool direct_operand(const T* p, long long ld, bool across, long long width, long long nr)
+static bool direct_operand(const T* p, long long ld, long long width)
 {
-    const long long n = Chunk<T>::N;
-    return (uintptr_t)p % 16 == 0 && ld % n == 0 && (across ? width : nr) % n == 0 && ld >= (across ? width : nr) &&
-           ld < (1LL << 21);
+    return (uintptr_t)p % 16 == 0 && ld % Chunk<T>::N == 0 && width % Chunk<T>::N == 0 && ld >= width && ld < (1LL << 21);
+}
+
+// Rows of an odd width are copied into rows of whole chunks first, zeros behind them, when the product is large against
+// the copies (two launches and two passes over the operands): 4099 x 1001 -> 2003 half precision 61 us through registers.
+static long long whole_chunks(long long width) { return (width + 7) / 8 * 8; }
+static bool pads(long long width, long long np, long long nq, long long nr, int dtype)
+{
+    return width % 8 != 0 && direct_sizes(np, nq, dtype) && (double)np * (double)nq * (double)nr >= 2147483648.0;
+}
+
+// (rows2 rows of a second matrix of the same width follow the first's)
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ from, long long ld, long long rows, int width,
+                                                       T* __restrict__ to, const T* __restrict__ from2, long long ld2,
+                                                       long long rows2)
+{
+    constexpr int N = Chunk<T>::N;
+    const int chunks = (width + N - 1) / N;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (rows + rows2) * chunks; i += (long long)gridDim.x * 256) {
+        const long long r = i / chunks;
+        const int c = (int)(i - r * chunks) * N;
+        const T* const row = r < rows ? from + r * ld : from2 + (r - rows) * ld2;
+        *(u32x4*)(to + r * chunks * N + c) = load16_head(row + c, width - c);
+    }
+}
+
+template <typename T>
+static void pad_rows(hipStream_t st, const T* from, long long ld, long long rows, int width, T* to,
+                     const T* from2 = nullptr, long long ld2 = 0, long long rows2 = 0)
+{
+    const long long blocks = ((rows + rows2) * ((width + 7) / 8) + 255) / 256;
+    hipLaunchKernelGGL(pad_rows_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, from, ld, rows,
+                       width, to, from2, ld2, rows2);
 }
 
 static size_t partial_bytes(long long np, long long nq, long long nr, int dtype)
@@ -488,8 +556,8 @@ static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partia
 {
     bool direct = false;
     if constexpr (sizeof(T) == 2)
-        direct = direct_sizes(a.np, a.nq, dtype) && direct_operand(a.p, a.ldp, PA, a.width_p, a.nr) &&
-                 direct_operand(a.q, a.ldq, QA, a.width_q, a.nr);
+        direct = direct_sizes(a.np, a.nq, dtype) && direct_operand(a.p, a.ldp, PA ? a.width_p : a.along) &&
+                 direct_operand(a.q, a.ldq, QA ? a.width_q : a.along);
     const Shape s = product_shape(a.np, a.nq, a.nr, dtype, direct);
     a.tiles_p = s.tiles_p;
     a.tiles_q = s.tiles_q;
@@ -524,14 +592,15 @@ static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partia
     return ngs_decoder_launched("ngs_linear");
 }
 
-static inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Backward workspace: dz (when there is an activation), the column sums' partials, the cut products' partials (the
 // two products run one after the other and share them).
 struct BackwardPlan {
     int across;
     long long col_blocks, row_blocks;
-    size_t sums_at, partial_at, total;
+    long long ldz;                       // elements between the rows of dz: n, or n in whole chunks
+    bool copy_dz, pad_w, pad_x;          // dz is made although it is dL_dy; weight and x are padded
+    size_t sums_at, partial_at, weight_at, x_at, total;
 };
 
 static BackwardPlan backward_plan(long long rows, int k, int n, int dtype, int act)
@@ -546,10 +615,17 @@ static BackwardPlan backward_plan(long long rows, int k, int n, int dtype, int a
     b.row_blocks = 2048 / (b.col_blocks > 0 ? b.col_blocks : 1);
     if (b.row_blocks > (rows + 4 * high - 1) / (4 * high)) b.row_blocks = (rows + 4 * high - 1) / (4 * high);
     if (b.row_blocks < 1) b.row_blocks = 1;
-    b.sums_at = act == NGS_ACT_NONE ? 0 : align256((size_t)rows * n * size);
+    const bool pad_z = pads(n, k, rows, n, dtype) || pads(n, k, n, rows, dtype);
+    b.ldz = pad_z ? whole_chunks(n) : n;
+    b.copy_dz = pad_z;
+    b.pad_w = pads(k, k, rows, n, dtype);
+    b.pad_x = pads(k, k, n, rows, dtype);
+    b.sums_at = act == NGS_ACT_NONE && !pad_z ? 0 : align256((size_t)rows * b.ldz * size);
     b.partial_at = b.sums_at + align256((size_t)b.row_blocks * n * 4);
     const size_t p1 = partial_bytes(k, rows, n, dtype), p2 = partial_bytes(k, n, rows, dtype);
-    b.total = b.partial_at + align256(p1 > p2 ? p1 : p2) + 256;
+    b.weight_at = b.partial_at + align256(p1 > p2 ? p1 : p2);
+    b.x_at = b.weight_at + (b.pad_w ? align256((size_t)n * whole_chunks(k) * size) : 0);
+    b.total = b.x_at + (b.pad_x ? align256((size_t)rows * whole_chunks(k) * size) : 0) + 256;
     return b;
 }
 
@@ -565,7 +641,7 @@ static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtyp
     a.ldq = ldx;
     a.np = n;
     a.nq = rows;
-    a.nr = k;
+    a.nr = a.along = k;
     a.epi.act = act;
     a.epi.bias = (const T*)bias;
     a.epi.residual = (const T*)res;
@@ -573,10 +649,22 @@ static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtyp
     a.epi.y = (T*)y;
     a.epi.slope = act == NGS_ACT_NONE ? nullptr : (typename Slope<T>::type*)slope;
     a.epi.np = n;
+    if (ngs_few_rows_takes(rows, k, n, dtype)) return ngs_few_rows<T>(st, rows, k, n, a.q, ldx, a.p, ldw, a.epi);
     if (ngs_stream_forward_takes(rows, k, n, dtype))
         return ngs_stream_forward<T>(st, rows, k, n, dtype, a.q, ldx, a.p, ldw, a.epi);
     a.width_p = n;
     a.width_q = rows;
+    if constexpr (sizeof(T) == 2) {
+        if (pads(k, n, rows, k, dtype)) {
+            const long long wide = whole_chunks(k);
+            T* const wp = (T*)(workspace + align256(partial_bytes(n, rows, k, dtype)));
+            T* const xp = wp + (size_t)n * wide;
+            pad_rows(st, a.p, ldw, n, k, wp, a.q, ldx, rows);
+            a.p = wp;
+            a.q = xp;
+            a.ldp = a.ldq = a.along = wide;
+        }
+    }
     return launch_product<T, false, false>(st, dtype, a, (float*)workspace);
 }
 
@@ -593,17 +681,17 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
     long long lddz = lddy;
     float* sums = (float*)(workspace + b.sums_at);
     float* partial = (float*)(workspace + b.partial_at);
-    const bool make_dz = act != NGS_ACT_NONE && (dx || dw) && rows > 0 && n > 0;
+    const bool make_dz = (act != NGS_ACT_NONE || b.copy_dz) && (dx || dw) && rows > 0 && n > 0;
     if (make_dz || db) {
         const dim3 grid((unsigned)b.row_blocks, (unsigned)b.col_blocks);
         hipLaunchKernelGGL(linear_dz_kernel<T>, grid, dim3(256), 0, st, rows, n, b.across, (const T*)dy, lddy,
                            act == NGS_ACT_NONE ? nullptr : (const typename Slope<T>::type*)slope,
-                           make_dz ? (T*)workspace : nullptr, db ? sums : nullptr);
+                           make_dz ? (T*)workspace : nullptr, b.ldz, db ? sums : nullptr);
         if (db) ngs_launch_column_finish(st, sums, b.row_blocks, n, 0, db, nullptr, dtype);
         if (ngs_decoder_launched("ngs_linear_backward")) return 1;
         if (make_dz) {
             dz = (const T*)workspace;
-            lddz = n;
+            lddz = b.ldz;
         }
     }
     if (dx) {
@@ -615,8 +703,16 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
         a.np = k;
         a.nq = rows;
         a.nr = n;
+        a.along = make_dz ? b.ldz : n;
         a.width_p = k;
         a.width_q = rows;
+        if constexpr (sizeof(T) == 2) {
+            if (b.pad_w) {
+                pad_rows(st, a.p, ldw, n, k, (T*)(workspace + b.weight_at));
+                a.p = (const T*)(workspace + b.weight_at);
+                a.ldp = a.width_p = whole_chunks(k);
+            }
+        }
         a.epi.y = (T*)dx;
         if (launch_product<T, true, false>(st, dtype, a, partial)) return 1;
     }
@@ -628,9 +724,16 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
         a.ldq = lddz;
         a.np = k;
         a.nq = n;
-        a.nr = rows;
+        a.nr = a.along = rows;
         a.width_p = k;
-        a.width_q = n;
+        a.width_q = make_dz ? b.ldz : n;
+        if constexpr (sizeof(T) == 2) {
+            if (b.pad_x) {
+                pad_rows(st, a.p, ldx, rows, k, (T*)(workspace + b.x_at));
+                a.p = (const T*)(workspace + b.x_at);
+                a.ldp = a.width_p = whole_chunks(k);
+            }
+        }
         a.epi.y = (T*)dw;
         if (launch_product<T, true, true>(st, dtype, a, partial)) return 1;
     }
@@ -652,8 +755,12 @@ static int check_linear(const char* what, long long rows, int k, int n, int dtyp
 extern "C" size_t ngs_linear_forward_workspace_bytes(long long rows, int in_features, int out_features, int dtype)
 {
     if (rows <= 0 || out_features <= 0 || in_features < 0 || rows > (1LL << 40) || !ngs_decoder_dtype(dtype)) return 0;
-    if (ngs_stream_forward_takes(rows, in_features, out_features, dtype)) return 0;
-    return partial_bytes(out_features, rows, in_features, dtype);
+    if (ngs_few_rows_takes(rows, in_features, out_features, dtype) ||
+        ngs_stream_forward_takes(rows, in_features, out_features, dtype))
+        return 0;
+    const size_t partial = partial_bytes(out_features, rows, in_features, dtype);
+    if (!pads(in_features, out_features, rows, in_features, dtype)) return partial;
+    return align256(partial) + (size_t)whole_chunks(in_features) * (rows + out_features) * ngs_decoder_size(dtype);
 }
 
 extern "C" int ngs_linear_forward(long long rows, int in_features, int out_features, int dtype, int activation,

@@ -10,6 +10,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 #define ROW_BYTES 128  // bytes of the reduction index that one step stages per row: 64 16-bit elements or 32 floats
 
 #define NGS_STREAM_ROWS 4096
+#define NGS_FEW_ROWS 64
 
 // Elements of the derivative array for T.
 template <typename T> struct Slope { typedef f16 type; };
@@ -249,3 +250,9 @@ template <typename T>
 int ngs_stream_backward(hipStream_t st, long long rows, int k, int n, int dtype, int act, const T* x, long long ldx,
                         const T* w, long long ldw, const T* bias, const T* dy, long long lddy, T* dx, T* dw, T* db,
                         float* partial);
+
+// linear_rows.hip: the product for a few rows
+bool ngs_few_rows_takes(long long rows, int k, int n, int dtype);
+template <typename T>
+int ngs_few_rows(hipStream_t st, long long rows, int k, int n, const T* x, long long ldx, const T* w, long long ldw,
+                 const Epilogue<T>& e);
