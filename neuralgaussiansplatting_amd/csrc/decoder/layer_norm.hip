@@ -9,7 +9,7 @@
 // rows a workgroup walks through; the workgroups' sums are joined in order by a second kernel.
 #include "decoder_common.h"
 
-#define NORM_WAVE_BLOCKS 2048  // workgroups of the kernels that give a row to a wave or less: what fills the chip
+#define NORM_WAVE_BLOCKS 1024  // workgroups of the kernels that give a row to a wave or less: what fills the chip
 
 template <int GROUP, int THREADS>
 struct Groups {
@@ -29,26 +29,58 @@ struct Groups {
         }
         return v;
     }
+    // two sums at once
+    static __device__ __forceinline__ void sum2(float& v, float& w, float* buf)
+    {
+#pragma unroll
+        for (int d = 1; d < (GROUP < 64 ? GROUP : 64); d <<= 1) {
+            v += __shfl_xor(v, d);
+            w += __shfl_xor(w, d);
+        }
+        if (GROUP > 64) {
+            const int wave = threadIdx.x >> 6;
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) {
+                buf[wave] = v;
+                buf[THREADS / 64 + wave] = w;
+            }
+            __syncthreads();
+            v = w = 0.0f;
+#pragma unroll
+            for (int k = 0; k < THREADS / 64; k++) {
+                v += buf[k];
+                w += buf[THREADS / 64 + k];
+            }
+        }
+    }
 };
 
-// The first `valid` of N weights as floats, `other` behind them and where there is no array.
+// A chunk's weights as they lie in memory (N of them: one or two 16-byte pieces), `other` where there is none: they stay
+// packed in registers between rows, which leaves room for the next row's loads.
 template <typename W, int N>
-__device__ __forceinline__ void load_weights(const W* p, long long at, int valid, float other, float (&f)[N])
-{
+struct Weights {
+    W e[N];
+    __device__ __forceinline__ void load(const W* p, long long at, long long valid, float other)
+    {
 #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = other;
-    if (!p || valid <= 0) return;
-    if (valid >= N) {
-        W e[N];
-        __builtin_memcpy(e, p + at, sizeof e);
+        for (int i = 0; i < N; i++) e[i] = (W)other;
+        if (!p || valid <= 0) return;
+        if (valid >= N) {
+            __builtin_memcpy(e, p + at, sizeof e);
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) f[i] = (float)e[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N - 1; i++)
-            if (i < valid) f[i] = (float)p[at + i];
+            for (int i = 0; i < N - 1; i++)
+                if (i < valid) e[i] = p[at + i];
+        }
     }
-}
+    __device__ __forceinline__ float operator[](int i) const { return (float)e[i]; }
+};
+
+// Whether a group has its next row on the way while it works on one: worth its registers for narrow rows and for groups
+// of several waves, which stand at barriers together; a lone wave with much to hold makes room for other waves instead
+// (100000 x 1024 bfloat16 there and back: 223 us ahead, 208 us not; 8191 x 5001 float16: 144 us and 172 us).
+template <int GROUP, int NC>
+constexpr bool norm_reads_ahead() { return GROUP <= 64 ? NC == 1 : GROUP < 1024; }
 
 template <typename T, typename W>
 struct NormArgs {
@@ -68,25 +100,37 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs<T, W> a)
     constexpr int N = Chunk<T>::N, SLOTS = THREADS / GROUP;
     __shared__ float buf[THREADS / 64];
     const int me = threadIdx.x % GROUP, slot = threadIdx.x / GROUP;
-    float w[NC][N], b[NC][N];
+    Weights<W, N> w[NC], b[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         const int col = (c * GROUP + me) * N;
-        load_weights<W, N>(a.weight, col, a.width - col, 1.0f, w[c]);
-        load_weights<W, N>(a.bias, col, a.width - col, 0.0f, b[c]);
+        w[c].load(a.weight, col, a.width - col, 1.0f);
+        b[c].load(a.bias, col, a.width - col, 0.0f);
     }
     // (a group without a row goes through the motions: the sums of a workgroup-wide group meet at barriers)
-    for (long long first = (long long)blockIdx.x * SLOTS; first < a.rows; first += (long long)gridDim.x * SLOTS) {
-        const long long row = first + slot;
-        const bool there = row < a.rows;
-        float v[NC][N], s = 0.0f;
+    u32x4 next[NC];
+    auto fetch = [&](long long row) {
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             const int col = (c * GROUP + me) * N;
-            unpack<T>(load16_head(a.x + row * a.ldx + col, there ? a.width - col : 0), v[c]);
+            next[c] = load16_head(a.x + row * a.ldx + col, row < a.rows ? a.width - col : 0);
+        }
+    };
+    constexpr bool AHEAD = norm_reads_ahead<GROUP, NC>();
+    const long long stride = (long long)gridDim.x * SLOTS;
+    long long first = (long long)blockIdx.x * SLOTS;
+    if (AHEAD) fetch(first + slot);
+    for (; first < a.rows; first += stride) {
+        const long long row = first + slot;
+        if (!AHEAD) fetch(row);
+        float v[NC][N], s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            unpack<T>(next[c], v[c]);
 #pragma unroll
             for (int i = 0; i < N; i++) s += v[c][i];
         }
+        if (AHEAD && first + stride < a.rows) fetch(row + stride);
         const float mean = Groups<GROUP, THREADS>::sum(s, buf) / a.width_f;
         s = 0.0f;
 #pragma unroll
@@ -99,7 +143,7 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormArgs<T, W> a)
             }
         }
         const float rstd = 1.0f / sqrtf(Groups<GROUP, THREADS>::sum(s, buf) / a.width_f + a.eps);
-        if (!there) continue;
+        if (row >= a.rows) continue;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             const int col = (c * GROUP + me) * N;
@@ -140,9 +184,9 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(NormArgs<T, W> 
     const float rstd = 1.0f / sqrtf(Groups<1024, 1024>::sum(s, buf) / a.width_f + a.eps);
     for (long long col = first; col < a.width; col += STEP) {
         const int valid = (int)(a.width - col < N ? a.width - col : N);
-        float w[N], b[N];
-        load_weights<W, N>(a.weight, col, valid, 1.0f, w);
-        load_weights<W, N>(a.bias, col, valid, 0.0f, b);
+        Weights<W, N> w, b;
+        w.load(a.weight, col, valid, 1.0f);
+        b.load(a.bias, col, valid, 0.0f);
         unpack<T>(load16_head(x + col, valid), f);
 #pragma unroll
         for (int i = 0; i < N; i++) f[i] = (f[i] - mean) * rstd * w[i] + b[i];
@@ -168,36 +212,47 @@ struct NormBackwardArgs {
 };
 
 template <typename T, typename W, int GROUP, int NC, int THREADS>
-__global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackwardArgs<T, W> a)
+__global__ __launch_bounds__(THREADS, THREADS <= 256 ? 2 : 1) void norm_backward_kernel(NormBackwardArgs<T, W> a)
 {
     constexpr int N = Chunk<T>::N, SLOTS = THREADS / GROUP;
-    __shared__ float buf[THREADS / 64];
+    __shared__ float buf[2 * (THREADS / 64)];
     __shared__ float join[SLOTS > 1 ? 2 * N * THREADS : 1];
     const int me = threadIdx.x % GROUP, slot = threadIdx.x / GROUP;
-    float w[NC][N], dw[NC][N], db[NC][N];
+    Weights<W, N> w[NC];
+    float dw[NC][N], db[NC][N];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         const int col = (c * GROUP + me) * N;
-        load_weights<W, N>(a.weight, col, a.width - col, 1.0f, w[c]);
+        w[c].load(a.weight, col, a.width - col, 1.0f);
 #pragma unroll
         for (int i = 0; i < N; i++) dw[c][i] = db[c][i] = 0.0f;
     }
-    for (long long first = (long long)blockIdx.x * SLOTS; first < a.rows; first += (long long)gridDim.x * SLOTS) {
+    u32x4 nx[NC], ng[NC];
+    float nmean = 0.0f, nrstd = 0.0f;
+    auto fetch = [&](long long row) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const int col = (c * GROUP + me) * N, valid = row < a.rows ? a.width - col : 0;
+            nx[c] = load16_head(a.x + row * a.ldx + col, valid);
+            ng[c] = load16_head(a.dy + row * a.lddy + col, valid);
+        }
+        nmean = row < a.rows ? a.mean[row] : 0.0f;
+        nrstd = row < a.rows ? a.rstd[row] : 0.0f;
+    };
+    constexpr bool AHEAD = norm_reads_ahead<GROUP, NC>();
+    const long long stride = (long long)gridDim.x * SLOTS;
+    long long first = (long long)blockIdx.x * SLOTS;
+    if (AHEAD) fetch(first + slot);
+    for (; first < a.rows; first += stride) {
         const long long row = first + slot;
         const bool there = row < a.rows;
-        const float mean = there ? a.mean[row] : 0.0f, rstd = there ? a.rstd[row] : 0.0f;
+        if (!AHEAD) fetch(row);
+        const float mean = nmean, rstd = nrstd;
         float u[NC][N], g[NC][N], sg = 0.0f, sgu = 0.0f;
-        u32x4 vx[NC], vg[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            const int col = (c * GROUP + me) * N, valid = there ? a.width - col : 0;
-            vx[c] = load16_head(a.x + row * a.ldx + col, valid);
-            vg[c] = load16_head(a.dy + row * a.lddy + col, valid);
-        }
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            unpack<T>(vx[c], u[c]);
-            unpack<T>(vg[c], g[c]);
+            unpack<T>(nx[c], u[c]);
+            unpack<T>(ng[c], g[c]);
             // (behind the row's end dy is zero, and u is of no account)
 #pragma unroll
             for (int i = 0; i < N; i++) {
@@ -209,9 +264,10 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackwardArgs
                 sgu += g[c][i] * u[c][i];
             }
         }
+        if (AHEAD && first + stride < a.rows) fetch(row + stride);
         if (!a.dx) continue;
-        const float mg = Groups<GROUP, THREADS>::sum(sg, buf) / a.width_f;
-        const float mgu = Groups<GROUP, THREADS>::sum(sgu, buf) / a.width_f;
+        Groups<GROUP, THREADS>::sum2(sg, sgu, buf);
+        const float mg = sg / a.width_f, mgu = sgu / a.width_f;
         if (!there) continue;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
@@ -239,6 +295,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackwardArgs
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 float sw = 0.0f, sb = 0.0f;
+#pragma unroll 4
                 for (int k = 0; k < SLOTS; k++) {
                     sw += join[i * THREADS + k * GROUP + me];
                     sb += join[(N + i) * THREADS + k * GROUP + me];
@@ -262,14 +319,15 @@ template <typename T, typename W>
 __global__ __launch_bounds__(1024) void norm_backward_wide_kernel(NormBackwardArgs<T, W> a)
 {
     constexpr int N = Chunk<T>::N, STEP = 1024 * N;
-    __shared__ float buf[16];
+    __shared__ float buf[32];
     const long long row = blockIdx.x;
     const T *const x = a.x + row * a.ldx, *const dy = a.dy + row * a.lddy;
     const float mean = a.mean[row], rstd = a.rstd[row];
     const int first = threadIdx.x * N;
-    float sg = 0.0f, sgu = 0.0f, u[N], g[N], w[N];
+    float sg = 0.0f, sgu = 0.0f, u[N], g[N];
+    Weights<W, N> w;
     for (long long col = first; col < a.width; col += STEP) {
-        load_weights<W, N>(a.weight, col, (int)(a.width - col < N ? a.width - col : N), 1.0f, w);
+        w.load(a.weight, col, a.width - col, 1.0f);
         unpack<T>(load16_head(x + col, a.width - col), u);
         unpack<T>(load16_head(dy + col, a.width - col), g);
 #pragma unroll
@@ -278,10 +336,10 @@ __global__ __launch_bounds__(1024) void norm_backward_wide_kernel(NormBackwardAr
             sgu += g[i] * w[i] * ((u[i] - mean) * rstd);
         }
     }
-    const float mg = Groups<1024, 1024>::sum(sg, buf) / a.width_f;
-    const float mgu = Groups<1024, 1024>::sum(sgu, buf) / a.width_f;
+    Groups<1024, 1024>::sum2(sg, sgu, buf);
+    const float mg = sg / a.width_f, mgu = sgu / a.width_f;
     for (long long col = first; col < a.width; col += STEP) {
-        load_weights<W, N>(a.weight, col, (int)(a.width - col < N ? a.width - col : N), 1.0f, w);
+        w.load(a.weight, col, a.width - col, 1.0f);
         unpack<T>(load16_head(x + col, a.width - col), u);
         unpack<T>(load16_head(dy + col, a.width - col), g);
 #pragma unroll
@@ -323,7 +381,7 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(NormBackwardArgs<T, W
 // ---------------------------------------------------------------------------
 // Launch shapes: threads per row and chunks per thread by the number of 16-byte chunks of a row
 // ---------------------------------------------------------------------------
-enum NormShape { G1, G2, G4, G8, G16, G32, G64, G64x2, G64x4, G256x2, G256x4, G1024x2, G1024x4, NORM_WIDE };
+enum NormShape { G1, G2, G4, G8, G16, G32, G64, G64x2, G64x3, G64x4, G256x2, G256x3, G256x4, G512x3, G512x4, G1024x3, G1024x4, NORM_WIDE };
 
 static NormShape norm_shape(long long width, int dtype)
 {
@@ -336,11 +394,16 @@ static NormShape norm_shape(long long width, int dtype)
     if (c <= 32) return G32;
     if (c <= 64) return G64;
     if (c <= 128) return G64x2;
+    if (c <= 192) return G64x3;
     if (c <= 256) return G64x4;
     if (c <= 512) return G256x2;
+    if (c <= 768) return G256x3;
     if (c <= 1024) return G256x4;
-    if (c <= 2048) return G1024x2;
-    if (c <= 4096) return G1024x4;
+    if (c <= 1536) return G512x3;
+    if (c <= 2048) return G512x4;
+    // (16-bit types hold twice as many elements per chunk: no registers for more)
+    if (dtype == NGS_FLOAT32 && c <= 3072) return G1024x3;
+    if (dtype == NGS_FLOAT32 && c <= 4096) return G1024x4;
     return NORM_WIDE;
 }
 
@@ -365,11 +428,19 @@ static long long norm_backward_blocks(long long rows, int width, int dtype)
     case G32: LAUNCH(32, 1, 256); break;          \
     case G64: LAUNCH(64, 1, 256); break;          \
     case G64x2: LAUNCH(64, 2, 256); break;        \
+    case G64x3: LAUNCH(64, 3, 256); break;        \
     case G64x4: LAUNCH(64, 4, 256); break;        \
     case G256x2: LAUNCH(256, 2, 256); break;      \
+    case G256x3: LAUNCH(256, 3, 256); break;      \
     case G256x4: LAUNCH(256, 4, 256); break;      \
-    case G1024x2: LAUNCH(1024, 2, 1024); break;   \
-    case G1024x4: LAUNCH(1024, 4, 1024); break;   \
+    case G512x3: LAUNCH(512, 3, 512); break;      \
+    case G512x4: LAUNCH(512, 4, 512); break;      \
+    case G1024x3:                                 \
+        if constexpr (sizeof(T) == 4) LAUNCH(1024, 3, 1024); \
+        break;                                    \
+    case G1024x4:                                 \
+        if constexpr (sizeof(T) == 4) LAUNCH(1024, 4, 1024); \
+        break;                                    \
     default: return ngs_set_error("ngs_layer_norm", "no kernel for this width"); \
     }
 
