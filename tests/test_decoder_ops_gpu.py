@@ -318,7 +318,7 @@ def test_norm_gradient_against_differences(ops):
 # ---- dropout ----
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("shape", [(1, 1), (7, 1), (1, 8), (3, 5), (64, 64), (13, 39), (2, 3, 10), (5, 1001), (9, 7)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (7, 1), (1, 8), (3, 5), (64, 64), (13, 39), (2, 3, 10), (5, 1001), (9, 7), (3, 2047), (2, 2049), (700, 39)], ids=str)
 def test_dropout_mask_and_values(ops, shape, dtype):
     g = gen(sum(shape))
     numel = torch.Size(shape).numel()
@@ -342,12 +342,15 @@ def test_dropout_strides_do_not_matter(ops, dtype):
     """The mask goes by an element's place among the rows, not by where it lies."""
     g = gen(1)
     wide, res = normal(g, 50, 64, dtype=dtype), normal(g, 50, 80, dtype=dtype)
-    for first, k in ((25, 39), (0, 24), (8, 40), (1, 63)):
+    for first, k in ((25, 39), (0, 24), (8, 40), (1, 63), (3, 1), (0, 2)):
         x, r = wide[:, first:first + k], res[:, first:first + k]
         want = ops.dropout(x.contiguous(), 0.3, 9, offset=2, residual=r.contiguous())
         assert torch.equal(ops.dropout(x, 0.3, 9, offset=2, residual=r), want)
         assert torch.equal(ops.dropout(x.contiguous(), 0.3, 9, offset=2, residual=r), want)
         assert torch.equal(ops.dropout(x.t().contiguous().t(), 0.3, 9, offset=2, residual=r), want)
+    for k in (2047, 2048, 2049, 5003):  # rows with gaps, about as long as what a workgroup takes
+        x = normal(g, 40, k + 2, dtype=dtype)[:, 1:k + 1]
+        assert torch.equal(ops.dropout(x, 0.3, 9, offset=2), ops.dropout(x.contiguous(), 0.3, 9, offset=2))
     row = normal(g, 40, dtype=dtype).expand(50, 40)
     assert torch.equal(ops.dropout(row, 0.3, 9), ops.dropout(row.contiguous(), 0.3, 9))
 
