@@ -15,6 +15,7 @@ import math
 import torch
 
 from .diff_gaussian_rasterization import GaussianRasterizationSettings, GaussianRasterizer
+from .rasterizer2 import GaussianRasterizationSettings2, GaussianRasterizer2
 from .sh_utils import eval_sh
 
 
@@ -77,3 +78,33 @@ def render(viewpoint_camera, pc, pipe, bg_color, scaling_modifier=1.0, override_
                                        rotations=rotations, cov3D_precomp=cov3D_precomp)
     return {"render": rendered_image, "viewspace_points": screenspace_points, "visibility_filter": radii > 0,
             "radii": radii}
+
+
+def render_features(viewpoint_camera, pc, decoder, pipe, bg_color, seed=0):
+    """Render through the index map and a decoder: every pixel's feature row (depth, encoded view direction, features
+    25..63 of the nearest Gaussian) is decoded to a colour; pixels that show no Gaussian get ``bg_color``.  The per-pixel
+    counterpart of the reference's neural front-end (gaussian_renderer/__init__.py:104-210).  ``pc`` also carries the
+    feature vectors ``_features`` [P, 64] (scene/gaussian_model.py:176), which receive gradients; ``decoder`` maps
+    [H, W, 64] and a dropout seed to [H, W, 3], e.g. a ``FeatureDecoder``.  Returns
+    ``{"render" [3, H, W], "idxmap", "depth", "feature_map"}``."""
+    settings = GaussianRasterizationSettings2(
+        image_height=int(viewpoint_camera.image_height),
+        image_width=int(viewpoint_camera.image_width),
+        tanfovx=math.tan(viewpoint_camera.FoVx * 0.5),
+        tanfovy=math.tan(viewpoint_camera.FoVy * 0.5),
+        bg=bg_color,
+        scale_modifier=1.0,
+        viewmatrix=viewpoint_camera.world_view_transform,
+        projmatrix=viewpoint_camera.full_proj_transform,
+        sh_degree=pc.active_sh_degree,
+        campos=viewpoint_camera.camera_center,
+        prefiltered=False,
+        debug=pipe.debug,
+    )
+    # (the index map takes its place from the centres alone and has gradients for the feature vectors alone)
+    xyz = pc.get_xyz.detach()
+    idxmap, _, depth, feature_map = GaussianRasterizer2(raster_settings=settings)(xyz, None, xyz, pc._features)
+    dtype = next((p.dtype for p in decoder.parameters()), feature_map.dtype)
+    colors = decoder(feature_map.to(dtype), seed).to(feature_map.dtype)
+    image = torch.where((idxmap >= 0).unsqueeze(-1), colors, bg_color.to(colors.dtype))
+    return {"render": image.permute(2, 0, 1), "idxmap": idxmap, "depth": depth, "feature_map": feature_map}
