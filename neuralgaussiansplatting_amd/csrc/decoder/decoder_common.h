@@ -34,6 +34,22 @@ __device__ __forceinline__ u32x4 load16(const T* p)
     return v;
 }
 
+// The same for 16-bit elements that may start in the middle of a word: the words they lie in, shifted into place.  A
+// 16-byte load that is not on a word's boundary takes the address unit several times as long (64 x 3711 -> 1000 bfloat16:
+// 58 us, against 20 us with 3710 or 3712 columns).  Every word that is read holds an element that was asked for.
+template <typename T>
+__device__ __forceinline__ u32x4 load16_any(const T* p)
+{
+    if constexpr (sizeof(T) != 2) return load16(p);
+    const uint32_t odd = ((uintptr_t)p >> 1) & 1;
+    const uint32_t* const words = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+    u32x4 v;
+    __builtin_memcpy(&v, words, 16);
+    const uint32_t last = words[3 + odd], s = odd * 16;
+    return (u32x4){__builtin_amdgcn_alignbit(v.y, v.x, s), __builtin_amdgcn_alignbit(v.z, v.y, s),
+                   __builtin_amdgcn_alignbit(v.w, v.z, s), __builtin_amdgcn_alignbit(last, v.w, s)};
+}
+
 // The first `valid` of the N elements at p (all, if that many or more; none, if <= 0), zeros behind them.
 template <typename T>
 __device__ __forceinline__ u32x4 load16_head(const T* p, long long valid)

@@ -13,15 +13,16 @@ struct FewRows {
     Epilogue<T> e;
 };
 
-// QF: fragments of 16 rows of x.  U: steps whose loads are on their way together.
-template <typename T, int QF>
+// QF: fragments of 16 rows of x.  ANY: some row starts in the middle of a word.  U: steps whose loads are on their way
+// together.
+template <typename T, int QF, bool ANY>
 __global__ __launch_bounds__(1024) void few_rows_kernel(FewRows<T> a)
 {
     constexpr int U = QF == 1 ? 8 : QF == 2 ? 4 : 2;
     extern __shared__ __attribute__((aligned(16))) f32x4 sums[];  // [wave][QF][lane]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, g = lane >> 4, i = lane & 15;
     const long long p = (long long)blockIdx.x * 16 + i;
-    const RowChunks<T> chunks(a.k);
+    const RowChunks<T, false, ANY> chunks(a.k);
     const T* const pw = a.w + (p < a.n ? p : a.n - 1) * a.ldw;
     const T* px[QF];
 #pragma unroll
@@ -76,7 +77,10 @@ __global__ __launch_bounds__(1024) void few_rows_kernel(FewRows<T> a)
 
 bool ngs_few_rows_takes(long long rows, int k, int n, int dtype)
 {
-    return rows >= 1 && rows <= NGS_FEW_ROWS && k >= 16 / (int)ngs_decoder_size(dtype) && n >= 1;
+    // (four fragments of rows and a long reduction: the tiles' second pass over the sums costs less than the waits here,
+    // 64 x 3712 -> 1000 bfloat16 20 us against 15 us; 64 x 1000 -> 1000 6 us against 12 us)
+    const int size = (int)ngs_decoder_size(dtype);
+    return rows >= 1 && (rows <= 32 || (rows <= NGS_FEW_ROWS && k <= 4096 / size)) && k >= 16 / size && n >= 1;
 }
 
 template <typename T, int QF>
@@ -88,7 +92,11 @@ static int few_rows_launch(hipStream_t st, FewRows<T> a)
     while (waves < 16 && (long long)groups * waves < 16 * NGS_CUS && steps >= 8 * waves) waves *= 2;
     a.run = (steps + waves - 1) / waves;
     const size_t lds = waves > 1 ? (size_t)waves * QF * 64 * sizeof(f32x4) : 0;
-    hipLaunchKernelGGL((few_rows_kernel<T, QF>), dim3(groups), dim3(64 * waves), lds, st, a);
+    const bool any = sizeof(T) == 2 && (((uintptr_t)a.x | (uintptr_t)a.w) & 3 || (a.ldx | a.ldw) & 1);
+    if constexpr (sizeof(T) == 2) {
+        if (any) hipLaunchKernelGGL((few_rows_kernel<T, QF, true>), dim3(groups), dim3(64 * waves), lds, st, a);
+    }
+    if (!any) hipLaunchKernelGGL((few_rows_kernel<T, QF, false>), dim3(groups), dim3(64 * waves), lds, st, a);
     return ngs_decoder_launched("ngs_linear_forward");
 }
 

@@ -17,8 +17,9 @@
 // ---------------------------------------------------------------------------
 // Rows in chunks.  A chunk that the row's end cuts is read from the end backwards and shifted into place, so that every
 // lane of a wave reads 16 bytes inside its row without a branch.  SHORT: rows of less than a chunk, read by elements.
+// ANY: rows that start in the middle of a word, as load16_any reads them.
 // ---------------------------------------------------------------------------
-template <typename T, bool SHORT = false>
+template <typename T, bool SHORT = false, bool ANY = false>
 struct RowChunks {
     int width, whole, tail;  // whole chunks, elements behind them
 
@@ -35,7 +36,7 @@ struct RowChunks {
             return u.v;
         }
         const int at = c * N < width - N ? c * N : width - N;
-        return load16(row + at);
+        return ANY ? load16_any(row + at) : load16(row + at);
     }
     // chunks first .. first + 3 are those of a step: what lies behind the row's end, or in no row, becomes zero
     __device__ __forceinline__ u32x4 settle(u32x4 v, int c, int first, bool there) const
@@ -89,13 +90,9 @@ struct WeightTile {
     static __device__ __forceinline__ void fill(char* lds, const T* __restrict__ w, long long ldw, int n, int k, int lines,
                                                 int tid, int threads)
     {
-        const RowChunks<T> rows(k);
         for (int i = tid; i < lines * CH; i += threads) {
             const int row = i / CH, c = i % CH;
-            u32x4 v = rows.fetch(w + (long long)(row < n ? row : n - 1) * ldw, c);
-            // (chunk by chunk: every chunk is the first of a "step" that may be cut)
-            v = rows.settle(v, c, c, row < n);
-            *(u32x4*)at(lds, row, c) = v;
+            *(u32x4*)at(lds, row, c) = load16_head(w + row * ldw + c * Chunk<T>::N, row < n ? k - c * Chunk<T>::N : 0);
         }
     }
     // the order in which fragment f takes 16 result columns: lane group g's four are neighbours, and for 16-bit types
@@ -156,10 +153,10 @@ struct StreamForward {
 };
 
 // KS: steps of four chunks that a row of x takes.  NB: groups of four chunks of the result that a workgroup computes
-// (blockIdx.y counts these).  A wave takes 16 rows at a time.  Loads and stores retire in order, so a row's results are
+// (blockIdx.y counts these).  SHORT: rows of x are shorter than a chunk.  A wave takes 16 rows at a time.  Loads and stores retire in order, so a row's results are
 // kept until the next rows have arrived: the wait for those then covers nothing younger, and both the stores and the
 // loads behind them have the whole computation of the next rows to get done.
-template <typename T, int KS, int NB, bool RESIDUAL, int THREADS>
+template <typename T, int KS, int NB, bool SHORT, bool RESIDUAL, int THREADS>
 __global__ __launch_bounds__(THREADS) void stream_forward_kernel(StreamForward<T> a)
 {
     constexpr int N = Chunk<T>::N, CH = KS * 4, PARTS = N / 4, COLS = NB * 4 * N;  // PARTS: fragments that make a chunk
@@ -174,7 +171,7 @@ __global__ __launch_bounds__(THREADS) void stream_forward_kernel(StreamForward<T
     for (int c = tid; c < COLS; c += THREADS) bias[c] = a.bias && c < n ? (float)a.bias[n0 + c] : 0.0f;
     __syncthreads();
 
-    const RowChunks<T> xc(a.k);
+    const RowChunks<T, SHORT> xc(a.k);
     const long long groups = (a.rows + 15) / 16, waves = (long long)gridDim.x * (THREADS / 64);
     long long group = (long long)blockIdx.x * (THREADS / 64) + (tid >> 6), done = -1;
     u32x4 nx[KS], nr[RESIDUAL ? NB : 1], y[NB];
@@ -265,15 +262,17 @@ struct StreamBackward {
     float* partial;  // [workgroup][n k + n]: sums for dW, then for db
 };
 
-// KS, NS: steps of four chunks that a row of x and of dz take; SHORT: rows of dz are shorter than a chunk.  As in the
+// KS, NS: steps of four chunks that a row of x and of dz take; SHORT_X, SHORT_Z: they are shorter than
+// a chunk.  As in the
 // forward pass, dx is kept until the next rows have arrived, where there are registers for it.
-template <typename T, int KS, int NS, bool SHORT, int WAVES>
+template <typename T, int KS, int NS, bool SHORT_X, bool SHORT_Z, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackward<T> a)
 {
     constexpr int N = Chunk<T>::N, CK = KS * 4, CN = NS * 4, PARTS = N / 4;
     constexpr int TK = CK * N, TN = CN * N, TM = WAVES * 16;          // columns of x, columns of dz, rows of a tile
     constexpr int FK = TK / 16, FN = TN / 16, EACH = (FK * FN + WAVES - 1) / WAVES;  // dW's fragments, and a wave's share:
-    constexpr int EK0 = EACH >= 8 ? 4 : EACH >= 2 ? 2 : 1, EK = EK0 < FK ? EK0 : FK, EN = EACH / EK;   // EK by EN of them
+    constexpr int EK0 = EACH >= 8 ? 4 : EACH >= 2 ? 2 : 1, EK1 = EK0 < FK ? EK0 : FK;
+    constexpr int EN = EACH / EK1 < FN ? EACH / EK1 : FN, EK = EACH / EN;   // EK by EN of them
     static_assert(FK % EK == 0 && FN % EN == 0, "shares fill dW");
     constexpr int STEPS = TM / (16 * PARTS);                          // reduction steps over a tile's rows
     typedef WeightTile<T, CK> W;
@@ -290,8 +289,8 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
     for (int c = tid; c < TN; c += 64 * WAVES) bias[c] = a.bias && c < a.n ? (float)a.bias[c] : 0.0f;
     __syncthreads();
 
-    const RowChunks<T> xc(a.k);
-    const RowChunks<T, SHORT> zc(a.n);
+    const RowChunks<T, SHORT_X> xc(a.k);
+    const RowChunks<T, SHORT_Z> zc(a.n);
     // db of 16-bit types gathers beside dz, unrounded; of floats it comes from the matrix units, as the product of ones
     // with the tile's dz, which costs a register per 16 columns and wave instead of N per step
     constexpr bool DB_MMA = sizeof(T) == 4;
@@ -472,6 +471,14 @@ inline int steps_of(long long width, int dtype)  // steps of four chunks, as a p
     return s;
 }
 
+// Backward: the product of x's and dz's steps that one workgroup's shared memory holds (the weight, and the tiles of 16
+// rows per wave), and the waves: eight, or four where a wave holds more than 256 registers' worth
+constexpr int stream_most(int size) { return size == 4 ? 64 : 32; }
+constexpr int stream_waves(int ks, int ns, int size)
+{
+    return ks * ns > 32 || ks > 8 || ns > 8 || (size == 2 && (ks > 4 || ns > 4)) ? 4 : 8;
+}
+
 // groups of four chunks of the result per workgroup: 1, 4 or 8
 inline int stream_blocks(int n, int dtype)
 {
@@ -479,7 +486,7 @@ inline int stream_blocks(int n, int dtype)
     return b <= 1 ? 1 : b <= 4 ? 4 : 8;
 }
 
-template <typename T, int KS, int NB, bool RESIDUAL>
+template <typename T, int KS, int NB, bool SHORT, bool RESIDUAL>
 static int stream_forward_launch(hipStream_t st, const StreamForward<T>& a)
 {
     constexpr int COLS = NB * 4 * Chunk<T>::N, LDS = COLS * (KS * 64 + 4);
@@ -487,16 +494,16 @@ static int stream_forward_launch(hipStream_t st, const StreamForward<T>& a)
     constexpr int PER_CU = 160 * 1024 / LDS < 2048 / THREADS ? 160 * 1024 / LDS : 2048 / THREADS;
     const long long need = ((a.rows + 15) / 16 + THREADS / 64 - 1) / (THREADS / 64), most = NGS_CUS * PER_CU;
     const dim3 grid((unsigned)(need < most ? need : most), (unsigned)((a.n + COLS - 1) / COLS));
-    hipLaunchKernelGGL((stream_forward_kernel<T, KS, NB, RESIDUAL, THREADS>), grid, dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((stream_forward_kernel<T, KS, NB, SHORT, RESIDUAL, THREADS>), grid, dim3(THREADS), 0, st, a);
     return ngs_decoder_launched("ngs_linear_forward");
 }
 
-template <typename T, int KS>
+template <typename T, int KS, bool SHORT = false>
 static int stream_forward_of(hipStream_t st, const StreamForward<T>& a, int dtype)
 {
     const int blocks = stream_blocks(a.n, dtype);
 #define NGS_STREAM_FORWARD(NB) \
-    (a.residual ? stream_forward_launch<T, KS, NB, true>(st, a) : stream_forward_launch<T, KS, NB, false>(st, a))
+    (a.residual ? stream_forward_launch<T, KS, NB, SHORT, true>(st, a) : stream_forward_launch<T, KS, NB, SHORT, false>(st, a))
     if (blocks == 1) return NGS_STREAM_FORWARD(1);
     // (eight steps and eight groups do not fit a wave's registers: the rows pass twice)
     if constexpr (KS < 8)
@@ -510,6 +517,7 @@ int ngs_stream_forward(hipStream_t st, long long rows, int k, int n, int dtype, 
                        long long ldw, const Epilogue<T>& e)
 {
     const StreamForward<T> a = {rows, k, n, x, w, e.bias, e.residual, ldx, ldw, e.ldr, e.act, e.y, e.slope};
+    if (k < Chunk<T>::N) return stream_forward_of<T, 1, true>(st, a, dtype);
     switch (steps_of(k, dtype)) {
     case 1: return stream_forward_of<T, 1>(st, a, dtype);
     case 2: return stream_forward_of<T, 2>(st, a, dtype);
@@ -518,27 +526,28 @@ int ngs_stream_forward(hipStream_t st, long long rows, int k, int n, int dtype, 
     }
 }
 
-template <typename T, int KS, int NS, bool SHORT = false>
+template <typename T, int KS, int NS, bool SHORT_X, bool SHORT_Z = false>
 static int stream_backward_launch(hipStream_t st, StreamBackward<T> a, unsigned blocks)
 {
-    constexpr int WAVES = KS * NS > 32 ? 4 : 8;
+    constexpr int WAVES = stream_waves(KS, NS, sizeof(T));
     a.tiles = (a.rows + WAVES * 16 - 1) / (WAVES * 16);
-    hipLaunchKernelGGL((stream_backward_kernel<T, KS, NS, SHORT, WAVES>), dim3(blocks), dim3(64 * WAVES), 0, st, a);
+    hipLaunchKernelGGL((stream_backward_kernel<T, KS, NS, SHORT_X, SHORT_Z, WAVES>), dim3(blocks), dim3(64 * WAVES), 0, st, a);
     return ngs_decoder_launched("ngs_linear_backward");
 }
 
-template <typename T, int KS>
+template <typename T, int KS, bool SHORT_X = false>
 static int stream_backward_of(hipStream_t st, const StreamBackward<T>& a, int ns, unsigned blocks)
 {
-    if (a.n < Chunk<T>::N) return stream_backward_launch<T, KS, 1, true>(st, a, blocks);
-    switch (ns) {
-    case 1: return stream_backward_launch<T, KS, 1>(st, a, blocks);
-    case 2: return stream_backward_launch<T, KS, 2>(st, a, blocks);
-    case 4: return stream_backward_launch<T, KS, 4>(st, a, blocks);
-    default:
-        if constexpr (sizeof(T) == 4) return stream_backward_launch<T, KS, 8>(st, a, blocks);
-        return ngs_set_error("ngs_linear_backward", "no kernel for this width");
-    }
+    constexpr int MOST = stream_most(sizeof(T)) / KS;  // steps of dz beside KS of x
+    if (a.n < Chunk<T>::N) return stream_backward_launch<T, KS, 1, SHORT_X, true>(st, a, blocks);
+    if (ns == 1) return stream_backward_launch<T, KS, 1, SHORT_X>(st, a, blocks);
+    if (ns == 2) return stream_backward_launch<T, KS, 2, SHORT_X>(st, a, blocks);
+    if (ns == 4) return stream_backward_launch<T, KS, 4, SHORT_X>(st, a, blocks);
+    if constexpr (MOST >= 8)
+        if (ns == 8) return stream_backward_launch<T, KS, 8, SHORT_X>(st, a, blocks);
+    if constexpr (MOST >= 16 && sizeof(T) == 4)
+        if (ns == 16) return stream_backward_launch<T, KS, 16, SHORT_X>(st, a, blocks);
+    return ngs_set_error("ngs_linear_backward", "no kernel for this width");
 }
 
 template <typename T>
@@ -549,13 +558,20 @@ int ngs_stream_backward(hipStream_t st, long long rows, int k, int n, int dtype,
     const StreamBackward<T> a = {rows, 0, k, n, x, w, bias, dy, ldx, ldw, lddy, act, dx, dw != nullptr, db != nullptr, partial};
     const unsigned blocks = (unsigned)ngs_stream_backward_blocks(rows, k, n, dtype);
     const int ns = steps_of(n, dtype);
+    const int ks = steps_of(k, dtype);
     int rc;
-    switch (steps_of(k, dtype)) {
-    case 1: rc = stream_backward_of<T, 1>(st, a, ns, blocks); break;
-    case 2: rc = stream_backward_of<T, 2>(st, a, ns, blocks); break;
-    case 4: rc = stream_backward_of<T, 4>(st, a, ns, blocks); break;
-    default:
-        if constexpr (sizeof(T) == 4) rc = stream_backward_of<T, 8>(st, a, ns, blocks);
+    if (k < Chunk<T>::N) {
+        rc = stream_backward_of<T, 1, true>(st, a, ns, blocks);
+    } else if (ks == 1) {
+        rc = stream_backward_of<T, 1>(st, a, ns, blocks);
+    } else if (ks == 2) {
+        rc = stream_backward_of<T, 2>(st, a, ns, blocks);
+    } else if (ks == 4) {
+        rc = stream_backward_of<T, 4>(st, a, ns, blocks);
+    } else if (ks == 8) {
+        rc = stream_backward_of<T, 8>(st, a, ns, blocks);
+    } else {
+        if constexpr (sizeof(T) == 4) rc = stream_backward_of<T, 16>(st, a, ns, blocks);
         else rc = ngs_set_error("ngs_linear_backward", "no kernel for this width");
     }
     if (rc) return rc;

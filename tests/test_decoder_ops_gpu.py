@@ -57,10 +57,12 @@ def check_linear(ops, rows, k, n, dtype, act, bias, residual, train=True, first=
 LINEAR_SIZES = [(1, 1, 1), (1, 64, 128), (3, 39, 3), (5, 17, 31), (16, 8, 40), (33, 100, 65), (127, 128, 129),
                 (128, 64, 128), (130, 200, 300), (257, 513, 40), (1000, 39, 3), (300, 1030, 520), (4100, 24, 16),
                 (2, 4096, 1000), (64, 5000, 48), (7, 3, 700), (40, 2050, 33), (2600, 128, 128), (2049, 64, 96), (8192, 64, 1024), (3000, 1000, 1000), (2048, 264, 3400), (600, 4104, 600), (2300, 1001, 1003), (1500, 1203, 1208), (1500, 1208, 1203),
-                (515, 256, 256), (9, 1027, 2051), (12, 512, 512), (1, 8192, 70), (4, 1111, 999), (8, 2048, 3), (15, 640, 4097), (16, 33, 5), (17, 700, 64),
+                (515, 256, 256), (9, 1027, 2051), (12, 512, 512), (1, 8192, 70), (4, 1111, 999), (8, 2048, 3), (15, 640, 4097), (16, 33, 5), (17, 700, 64), (33, 1001, 50), (64, 3711, 40), (60, 9, 17),
                 # many narrow rows
                 (4096, 1, 1), (4097, 3, 5), (5000, 39, 3), (4999, 128, 128), (4100, 127, 129), (6001, 200, 24), (4200, 17, 100),
-                (4111, 256, 40), (9000, 64, 128), (4500, 8, 250), (5003, 65, 33), (4099, 33, 64), (70001, 40, 48)]
+                (4111, 256, 40), (9000, 64, 128), (4500, 8, 250), (5003, 65, 33), (4099, 33, 64), (70001, 40, 48), (4100, 2, 70),
+                (4101, 7, 7), (5000, 3, 2), (4300, 100, 200), (4400, 250, 60), (4200, 60, 255), (4150, 256, 3), (4160, 3, 256),
+                (4170, 130, 256), (8300, 16, 152)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -86,7 +88,7 @@ def test_linear_activations(ops, size, act, dtype):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("case", [(300, 39, 3, 25, 64), (2500, 39, 64, 25, 64), (1, 39, 20, 25, 64), (140, 128, 130, 8, 144),
                                   (300, 63, 64, 1, 65), (5, 256, 32, 0, 300), (5000, 39, 64, 25, 64), (4500, 39, 3, 25, 64),
-                                  (4501, 128, 128, 0, 130), (4502, 63, 30, 1, 67)], ids=str)
+                                  (4501, 128, 128, 0, 130), (4502, 63, 30, 1, 67), (4503, 5, 72, 25, 30)], ids=str)
 def test_linear_slices(ops, case, dtype):
     """Rows that are slices of wider ones (the 39 copied features of a feature row), aligned or not."""
     rows, k, n, first, pitch = case
