@@ -201,8 +201,8 @@ struct TileLoader {
 
 // A wave's results through its own piece of shared memory, 16 rows at a time, so that they leave as whole lines and the
 // epilogue's code is there once per 16 rows rather than once per fragment.  BARE: no epilogue.
-template <int MP>
-constexpr int finish_wide_bytes() { return 16 * (MP * 16 + 4) * 4 + 16 * MP * 16 * 2; }  // a wave's piece
+template <typename T, int MP>
+constexpr int finish_wide_bytes() { return 16 * (MP * 16 + 4) * 4 + 16 * MP * 16 * (int)sizeof(T); }  // a wave's piece
 
 template <typename T, int MP, int MQ, bool BARE>
 __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&acc)[MP][MQ], float* lds, long long p0,
@@ -339,8 +339,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_direct_kernel(Product<T>
         buf ^= 1;
     }
     __syncthreads();  // the tiles are done with
-    static_assert(WAVES * finish_wide_bytes<MP>() <= 2 * STAGE, "a piece of the tiles' memory for each wave");
-    finish_wide<T, MP, MQ, P_ACROSS>(a, acc, (float*)(lds + wave * finish_wide_bytes<MP>()), at.p0 + wp * MP * 16, at.q0 + wq * MQ * 16,
+    static_assert(WAVES * finish_wide_bytes<T, MP>() <= 2 * STAGE, "a piece of the tiles' memory for each wave");
+    finish_wide<T, MP, MQ, P_ACROSS>(a, acc, (float*)(lds + wave * finish_wide_bytes<T, MP>()), at.p0 + wp * MP * 16, at.q0 + wq * MQ * 16,
                                      at.split, lane);
 }
 
@@ -461,6 +461,7 @@ struct Shape {
     long long tiles_p, tiles_q;
     int splits;
     long long run;
+    static long long tiles(long long np, long long nq, long long t) { return ((np + t - 1) / t) * ((nq + t - 1) / t); }
     long long groups() const { return (tiles_p * tiles_q * splits + NGS_XCDS - 1) / NGS_XCDS * NGS_XCDS; }
     size_t partial_bytes(long long np, long long nq) const { return splits > 1 ? (size_t)splits * np * nq * 4 : 0; }
 };
@@ -469,7 +470,7 @@ static inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Through registers, tiles are 128 wide unless the matrix is 32 or narrower; a reduction is cut until the tiles and its
 // runs fill the chip twice, each run at least four steps long.
-// Directly (16-bit types), tiles are 256 x 256, one to a compute unit, or 128 x 128, two at a time.  A round of the
+// Directly, tiles of 16-bit types are 256 x 256, one to a compute unit, or 128 x 128, two at a time.  A round of the
 // former takes one and a half times as long as one of the latter (8192 x 4096 -> 4096 bfloat16: 2 rounds 233 us, 4 rounds
 // 317 us; 6144 x 1024 -> 3200: 2 rounds 64 us, 2.3 rounds 51 us; 4096 x 1024 -> 2048: 35 us and 24 us, one round each); a
 // last round of small tiles that does not fill the chip costs about 0.6 of a full one.
@@ -478,7 +479,10 @@ static Shape product_shape(long long np, long long nq, long long nr, int dtype, 
     Shape s;
     s.tp = np <= 32 ? 32 : 128;
     s.tq = nq <= 32 ? 32 : 128;
-    if (direct) {
+    if (direct && dtype == NGS_FLOAT32) {
+        // the matrix units bound either tile: the small one shares the work out more evenly
+        if (s.tiles(np, nq, 128) < 4 * NGS_CUS) s.tp = s.tq = 64;
+    } else if (direct) {
         const long long large = ((np + 255) / 256) * ((nq + 255) / 256), small = ((np + 127) / 128) * ((nq + 127) / 128);
         const double large_cost = 1.5 * (double)((large + NGS_CUS - 1) / NGS_CUS);
         const double small_cost = (double)(small / (2 * NGS_CUS)) + (small % (2 * NGS_CUS) ? 0.6 : 0.0);
@@ -501,7 +505,7 @@ static Shape product_shape(long long np, long long nq, long long nr, int dtype, 
 }
 
 // Whether product_direct_kernel has a tile for these sizes
-static bool direct_sizes(long long np, long long nq, int dtype) { return dtype != NGS_FLOAT32 && np > 32 && nq > 32; }
+static bool direct_sizes(long long np, long long nq) { return np > 32 && nq > 32; }
 
 // Whether it can read an operand: whole aligned chunks, and offsets within a tile's rows in 31 bits
 template <typename T>
@@ -512,10 +516,15 @@ static bool direct_operand(const T* p, long long ld, long long width)
 
 // Rows of an odd width are copied into rows of whole chunks first, zeros behind them, when the product is large against
 // the copies (two launches and two passes over the operands): 4099 x 1001 -> 2003 half precision 61 us through registers.
-static long long whole_chunks(long long width) { return (width + 7) / 8 * 8; }
+static long long whole_chunks(long long width, int dtype)
+{
+    const long long n = 16 / (long long)ngs_decoder_size(dtype);
+    return (width + n - 1) / n * n;
+}
 static bool pads(long long width, long long np, long long nq, long long nr, int dtype)
 {
-    return width % 8 != 0 && direct_sizes(np, nq, dtype) && (double)np * (double)nq * (double)nr >= 2147483648.0;
+    return width != whole_chunks(width, dtype) && direct_sizes(np, nq) &&
+           (double)np * (double)nq * (double)nr >= (dtype == NGS_FLOAT32 ? 268435456.0 : 2147483648.0);
 }
 
 // (rows2 rows of a second matrix of the same width follow the first's)
@@ -538,7 +547,7 @@ template <typename T>
 static void pad_rows(hipStream_t st, const T* from, long long ld, long long rows, int width, T* to,
                      const T* from2 = nullptr, long long ld2 = 0, long long rows2 = 0)
 {
-    const long long blocks = ((rows + rows2) * ((width + 7) / 8) + 255) / 256;
+    const long long blocks = ((rows + rows2) * ((width + Chunk<T>::N - 1) / Chunk<T>::N) + 255) / 256;
     hipLaunchKernelGGL(pad_rows_kernel<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, from, ld, rows,
                        width, to, from2, ld2, rows2);
 }
@@ -546,7 +555,7 @@ static void pad_rows(hipStream_t st, const T* from, long long ld, long long rows
 static size_t partial_bytes(long long np, long long nq, long long nr, int dtype)
 {
     const size_t a = product_shape(np, nq, nr, dtype, false).partial_bytes(np, nq);
-    if (!direct_sizes(np, nq, dtype)) return a;
+    if (!direct_sizes(np, nq)) return a;
     const size_t b = product_shape(np, nq, nr, dtype, true).partial_bytes(np, nq);
     return a > b ? a : b;
 }
@@ -554,9 +563,7 @@ static size_t partial_bytes(long long np, long long nq, long long nr, int dtype)
 template <typename T, bool PA, bool QA>
 static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partial)
 {
-    bool direct = false;
-    if constexpr (sizeof(T) == 2)
-        direct = direct_sizes(a.np, a.nq, dtype) && direct_operand(a.p, a.ldp, PA ? a.width_p : a.along) &&
+    const bool direct = direct_sizes(a.np, a.nq) && direct_operand(a.p, a.ldp, PA ? a.width_p : a.along) &&
                  direct_operand(a.q, a.ldq, QA ? a.width_q : a.along);
     const Shape s = product_shape(a.np, a.nq, a.nr, dtype, direct);
     a.tiles_p = s.tiles_p;
@@ -567,13 +574,13 @@ static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partia
     a.epi.partial = s.splits > 1 ? partial : nullptr;
     if (s.groups() > 0x7fffffffLL) return ngs_set_error("ngs_linear", "too many rows");
     const dim3 grid((unsigned)s.groups());
-    if constexpr (sizeof(T) == 2) {
-        if (direct && s.tp == 256)
+    if (direct && s.tp == 128) {
+        hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
+    } else if (direct) {
+        if constexpr (sizeof(T) == 2)
             hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 256, 256, 2, 4>), grid, dim3(512), 0, st, a);
-        else if (direct)
-            hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
-    }
-    if (direct) {
+        else
+            hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 64, 64, 2, 2>), grid, dim3(256), 0, st, a);
     } else if (s.tp == 128 && s.tq == 128) {
         hipLaunchKernelGGL((product_kernel<T, PA, QA, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
     } else if (s.tp == 128) {
@@ -616,7 +623,7 @@ static BackwardPlan backward_plan(long long rows, int k, int n, int dtype, int a
     if (b.row_blocks > (rows + 4 * high - 1) / (4 * high)) b.row_blocks = (rows + 4 * high - 1) / (4 * high);
     if (b.row_blocks < 1) b.row_blocks = 1;
     const bool pad_z = pads(n, k, rows, n, dtype) || pads(n, k, n, rows, dtype);
-    b.ldz = pad_z ? whole_chunks(n) : n;
+    b.ldz = pad_z ? whole_chunks(n, dtype) : n;
     b.copy_dz = pad_z;
     b.pad_w = pads(k, k, rows, n, dtype);
     b.pad_x = pads(k, k, n, rows, dtype);
@@ -624,8 +631,8 @@ static BackwardPlan backward_plan(long long rows, int k, int n, int dtype, int a
     b.partial_at = b.sums_at + align256((size_t)b.row_blocks * n * 4);
     const size_t p1 = partial_bytes(k, rows, n, dtype), p2 = partial_bytes(k, n, rows, dtype);
     b.weight_at = b.partial_at + align256(p1 > p2 ? p1 : p2);
-    b.x_at = b.weight_at + (b.pad_w ? align256((size_t)n * whole_chunks(k) * size) : 0);
-    b.total = b.x_at + (b.pad_x ? align256((size_t)rows * whole_chunks(k) * size) : 0) + 256;
+    b.x_at = b.weight_at + (b.pad_w ? align256((size_t)n * whole_chunks(k, dtype) * size) : 0);
+    b.total = b.x_at + (b.pad_x ? align256((size_t)rows * whole_chunks(k, dtype) * size) : 0) + 256;
     return b;
 }
 
@@ -654,16 +661,14 @@ static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtyp
         return ngs_stream_forward<T>(st, rows, k, n, dtype, a.q, ldx, a.p, ldw, a.epi);
     a.width_p = n;
     a.width_q = rows;
-    if constexpr (sizeof(T) == 2) {
-        if (pads(k, n, rows, k, dtype)) {
-            const long long wide = whole_chunks(k);
-            T* const wp = (T*)(workspace + align256(partial_bytes(n, rows, k, dtype)));
-            T* const xp = wp + (size_t)n * wide;
-            pad_rows(st, a.p, ldw, n, k, wp, a.q, ldx, rows);
-            a.p = wp;
-            a.q = xp;
-            a.ldp = a.ldq = a.along = wide;
-        }
+    if (pads(k, n, rows, k, dtype)) {
+        const long long wide = whole_chunks(k, dtype);
+        T* const wp = (T*)(workspace + align256(partial_bytes(n, rows, k, dtype)));
+        T* const xp = wp + (size_t)n * wide;
+        pad_rows(st, a.p, ldw, n, k, wp, a.q, ldx, rows);
+        a.p = wp;
+        a.q = xp;
+        a.ldp = a.ldq = a.along = wide;
     }
     return launch_product<T, false, false>(st, dtype, a, (float*)workspace);
 }
@@ -706,12 +711,10 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
         a.along = make_dz ? b.ldz : n;
         a.width_p = k;
         a.width_q = rows;
-        if constexpr (sizeof(T) == 2) {
-            if (b.pad_w) {
-                pad_rows(st, a.p, ldw, n, k, (T*)(workspace + b.weight_at));
-                a.p = (const T*)(workspace + b.weight_at);
-                a.ldp = a.width_p = whole_chunks(k);
-            }
+        if (b.pad_w) {
+            pad_rows(st, a.p, ldw, n, k, (T*)(workspace + b.weight_at));
+            a.p = (const T*)(workspace + b.weight_at);
+            a.ldp = a.width_p = whole_chunks(k, dtype);
         }
         a.epi.y = (T*)dx;
         if (launch_product<T, true, false>(st, dtype, a, partial)) return 1;
@@ -727,12 +730,10 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
         a.nr = a.along = rows;
         a.width_p = k;
         a.width_q = make_dz ? b.ldz : n;
-        if constexpr (sizeof(T) == 2) {
-            if (b.pad_x) {
-                pad_rows(st, a.p, ldx, rows, k, (T*)(workspace + b.x_at));
-                a.p = (const T*)(workspace + b.x_at);
-                a.ldp = a.width_p = whole_chunks(k);
-            }
+        if (b.pad_x) {
+            pad_rows(st, a.p, ldx, rows, k, (T*)(workspace + b.x_at));
+            a.p = (const T*)(workspace + b.x_at);
+            a.ldp = a.width_p = whole_chunks(k, dtype);
         }
         a.epi.y = (T*)dw;
         if (launch_product<T, true, true>(st, dtype, a, partial)) return 1;
@@ -760,7 +761,7 @@ extern "C" size_t ngs_linear_forward_workspace_bytes(long long rows, int in_feat
         return 0;
     const size_t partial = partial_bytes(out_features, rows, in_features, dtype);
     if (!pads(in_features, out_features, rows, in_features, dtype)) return partial;
-    return align256(partial) + (size_t)whole_chunks(in_features) * (rows + out_features) * ngs_decoder_size(dtype);
+    return align256(partial) + (size_t)whole_chunks(in_features, dtype) * (rows + out_features) * ngs_decoder_size(dtype);
 }
 
 extern "C" int ngs_linear_forward(long long rows, int in_features, int out_features, int dtype, int activation,

@@ -18,7 +18,8 @@ bool ngs_stream_backward_takes(long long rows, int k, int n, int dtype)
 {
     if (rows < NGS_STREAM_ROWS || k < 1 || n < 1) return false;
     const int size = (int)ngs_decoder_size(dtype), ks = steps_of(k, dtype), ns = steps_of(n, dtype);
-    return ks <= 32 / size && ns <= 32 / size && ks * ns <= stream_most(size);
+    return ks <= 4 * size && ns <= 4 * size && ks * ns <= stream_most(size);  // a width of 256
+
 }
 
 long long ngs_stream_backward_blocks(long long rows, int k, int n, int dtype)
