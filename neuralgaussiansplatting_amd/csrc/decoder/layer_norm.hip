@@ -485,7 +485,7 @@ static int norm_backward(hipStream_t st, int dtype, int weight_dtype, NormBackwa
 static int check_norm(const char* what, long long rows, int width, int dtype, int weight_dtype)
 {
     if (rows < 0 || width < 0) return ngs_set_error(what, "a size is negative");
-    if (rows > (1LL << 40)) return ngs_set_error(what, "too many rows");
+    if (rows > (1LL << 40) || (double)rows * width > 281474976710656.0) return ngs_set_error(what, "too many elements");
     if (!ngs_decoder_dtype(dtype) || !ngs_decoder_dtype(weight_dtype)) return ngs_set_error(what, "unknown element type");
     if (weight_dtype != dtype && weight_dtype != NGS_FLOAT32)
         return ngs_set_error(what, "the weights must be of the rows' type or float32");

@@ -744,10 +744,16 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
 // ---------------------------------------------------------------------------
 // C entry points
 // ---------------------------------------------------------------------------
+// (byte counts of operands and workspaces stay far from 64 bits)
+static bool too_many(long long rows, int k, int n)
+{
+    return rows > (1LL << 40) || (double)rows * (k > n ? k : n) > 281474976710656.0;
+}
+
 static int check_linear(const char* what, long long rows, int k, int n, int dtype, int act)
 {
     if (rows < 0 || k < 0 || n < 0) return ngs_set_error(what, "a size is negative");
-    if (rows > (1LL << 40)) return ngs_set_error(what, "too many rows");
+    if (too_many(rows, k, n)) return ngs_set_error(what, "too many elements");
     if (!ngs_decoder_dtype(dtype)) return ngs_set_error(what, "unknown element type");
     if (act < NGS_ACT_NONE || act > NGS_ACT_SIGMOID) return ngs_set_error(what, "unknown activation");
     return 0;
@@ -755,7 +761,9 @@ static int check_linear(const char* what, long long rows, int k, int n, int dtyp
 
 extern "C" size_t ngs_linear_forward_workspace_bytes(long long rows, int in_features, int out_features, int dtype)
 {
-    if (rows <= 0 || out_features <= 0 || in_features < 0 || rows > (1LL << 40) || !ngs_decoder_dtype(dtype)) return 0;
+    if (rows <= 0 || out_features <= 0 || in_features < 0 || too_many(rows, in_features, out_features) ||
+        !ngs_decoder_dtype(dtype))
+        return 0;
     if (ngs_few_rows_takes(rows, in_features, out_features, dtype) ||
         ngs_stream_forward_takes(rows, in_features, out_features, dtype))
         return 0;
@@ -799,7 +807,9 @@ extern "C" int ngs_linear_backward_reads_slope(long long rows, int in_features, 
 extern "C" size_t ngs_linear_backward_workspace_bytes(long long rows, int in_features, int out_features, int dtype,
                                                       int activation)
 {
-    if (rows < 0 || in_features < 0 || out_features < 0 || rows > (1LL << 40) || !ngs_decoder_dtype(dtype)) return 0;
+    if (rows < 0 || in_features < 0 || out_features < 0 || too_many(rows, in_features, out_features) ||
+        !ngs_decoder_dtype(dtype))
+        return 0;
     if (ngs_stream_backward_takes(rows, in_features, out_features, dtype))
         return (size_t)ngs_stream_backward_blocks(rows, in_features, out_features, dtype) *
                ((size_t)in_features * out_features + out_features) * sizeof(float);

@@ -369,8 +369,11 @@ __global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackw
                             for (int e = 0; e < 4; e++) z[h * 4 + e] = c[e];
                         }
                         activate<N>(a.act, z, y, slope);
+                        // (behind the last column z may be NaN where x is not finite, and must not reach dx)
+                        const int left = a.n - (s * 4 + g) * N;
+                        const bool whole = (s * 4 + 4) * N <= a.n;  // uniform
 #pragma unroll
-                        for (int e = 0; e < N; e++) d[e] *= slope[e];
+                        for (int e = 0; e < N; e++) d[e] = whole || e < left ? d[e] * slope[e] : 0.0f;
                         dz[s] = pack<T>(d);
                     }
                     if constexpr (!DB_MMA) {

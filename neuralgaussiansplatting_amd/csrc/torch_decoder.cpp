@@ -106,6 +106,22 @@ void refuse_double_backward(const char* what)
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative (create_graph=True)");
 }
 
+// A gradient's accumulator belongs to the stream it was made on.  One that an earlier, eager graph of the same leaf keeps
+// alive would make the backward pass wait across streams, which a capture does not survive: refused here, where it can
+// still be told.
+void check_capture(const char* what, const c10::optional<Tensor>& t)
+{
+    if (!wants_grad(t) || !t->is_leaf()) return;
+    const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t->device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!accumulator) return;
+    const auto its = accumulator->stream();
+    TORCH_CHECK(!its.has_value() || *its == stream.unwrap(), what,
+                ": cannot be captured with gradients while an earlier graph of the same tensor is alive (drop its outputs first)");
+}
+
 // ---- linear ----
 
 int activation_of(const std::string& name)
@@ -214,8 +230,10 @@ Tensor linear(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>
         check_like("linear", "residual", *residual, x);
         TORCH_CHECK(residual->sizes().vec() == with_last(x, weight.size(0)), "linear: residual must have the output's dimensions");
     }
-    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(bias) || wants_grad(residual)))
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(bias) || wants_grad(residual))) {
+        for (const auto& t : {c10::optional<Tensor>(x), c10::optional<Tensor>(weight), bias, residual}) check_capture("linear", t);
         return LinearFunction::apply(x, weight, bias, (int64_t)act, residual);
+    }
     return linear_run(x, weight, bias, act, residual, nullptr);
 }
 
@@ -300,8 +318,10 @@ Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight, const c1
     TORCH_CHECK(!weight.has_value() || !bias.has_value() || weight->scalar_type() == bias->scalar_type(),
                 "layer_norm: weight and bias must have the same type");
     TORCH_CHECK(eps >= 0, "layer_norm: eps must not be negative");
-    if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))
+    if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias))) {
+        for (const auto& t : {c10::optional<Tensor>(x), weight, bias}) check_capture("layer_norm", t);
         return LayerNormFunction::apply(x, weight, bias, eps);
+    }
     return norm_run(x, weight, bias, eps, nullptr);
 }
 
@@ -377,8 +397,10 @@ Tensor dropout(const Tensor& x, double p, const pybind11::object& seed, const py
         TORCH_CHECK(residual->sizes() == x.sizes(), "dropout: residual must have the dimensions of x");
     }
     const pybind11::gil_scoped_release release;
-    if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual)))
+    if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual))) {
+        for (const auto& t : {c10::optional<Tensor>(x), residual}) check_capture("dropout", t);
         return DropoutFunction::apply(x, p, seed_word, seed_tensor, offset_word, residual);
+    }
     return dropout_run(x, p, seed_word, seed_tensor, offset_word, residual);
 }
 

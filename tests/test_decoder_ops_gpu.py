@@ -545,6 +545,57 @@ def test_captured_and_replayed(ops):
             assert torch.equal(a, b), i
 
 
+def test_capture_refuses_a_leaf_of_a_living_graph(ops):
+    """A gradient's accumulator that an eager graph keeps alive belongs to that graph's stream; a captured backward pass
+    would have to wait for it across streams.  Refused in the forward call, before anything is captured."""
+    x = torch.ones(8, 8, device=DEV, requires_grad=True)
+    w = torch.ones(8, 8, device=DEV)
+    calls = [lambda: ops.linear(x, w), lambda: ops.layer_norm(x), lambda: ops.dropout(x, 0.5, 1)]
+    for call in calls:
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="graph of the same tensor is alive"):
+            with torch.cuda.graph(graph):
+                torch.zeros(1, device=DEV)  # (an empty capture would warn)
+                call()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call()
+            (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call()
+        assert torch.equal(y.detach(), want.detach())
+        assert torch.equal(dx, torch.autograd.grad(want, [x], torch.ones_like(want))[0])
+        del y, dx, want
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows", [300, 4200])
+def test_linear_gradients_beside_infinities(ops, rows, dtype):
+    """Where the derivative is finite although z is not (relu, sigmoid), so are the gradients, at widths that fill no
+    step; rows without infinities do not notice."""
+    for k, n in ((40, 17), (17, 3), (24, 40)):
+        g = gen(n)
+        x, w = normal(g, rows, k, dtype=dtype), normal(g, n, k, dtype=dtype)
+        w[w == 0] = 1
+        x[7, 2], x[rows - 1, k - 1] = float("inf"), -float("inf")
+        dy = torch.randint(-3, 4, (rows, n), generator=g, device=DEV).to(dtype)
+        for act in ("relu", "sigmoid"):
+            xl = x.clone().requires_grad_()
+            y = ops.linear(xl, w, activation=act)
+            (dx,) = torch.autograd.grad(y, [xl], dy)
+            assert torch.isfinite(dx).all()
+            for r, c in ((7, 2), (rows - 1, k - 1)):
+                up = (w[:, c] > 0) == (x[r, c] > 0)  # z = +inf there, -inf elsewhere
+                assert torch.equal(y[r], torch.where(up, float("inf") if act == "relu" else 1.0, 0.0).to(dtype))
+                slope = up.double() if act == "relu" else torch.zeros(n, device=DEV, dtype=torch.float64)
+                want = (dy[r].double() * slope) @ w.double()
+                bound = (n + 2) * 2 * ref.E * ((dy[r].double() * slope).abs() @ w.double().abs())
+                ref.assert_within(dx[r], (want, ref.rounded(want, bound, dtype)), act)
+
+
 def test_far_offsets(ops):
     """More than 2^31 elements: the last rows come out as they do on their own."""
     rows, d = (1 << 21) + 300, 1032
