@@ -23,54 +23,72 @@ struct Product {
     // nq columns; of one that lies along, the reduction's nr
     long long width_p, width_q, along;
     long long tiles_p, tiles_q;
-    int splits;          // the reduction is cut into this many runs of `run` elements (a multiple of a step's)
-    long long run;
+    // The first `full` tiles are computed whole, by `full_groups` workgroups (a multiple of the dies); each of the others
+    // by `parts` workgroups, which take `run` elements of the reduction each (a multiple of a step's) and, if there is
+    // more than one, leave their sums in partial[workgroup][q in tile][p in tile].
+    long long full, full_groups, run;
+    int parts;
+    float* partial;
     Epilogue<T> epi;
 };
 
 // Which tile and which run of the reduction a workgroup computes.  Workgroups go to the dies in turn: each die takes a
-// contiguous run of tiles, whose operands meet in its cache.
+// contiguous run of the whole tiles, whose operands meet in its cache.
 struct Place {
-    long long p0, q0, split, r_begin, r_end;
+    long long p0, q0, r_begin, r_end;
+    float* partial;  // where the sums go, if the tile is shared
     bool there;
 };
 template <typename T, int TP, int TQ>
 __device__ __forceinline__ Place place_of(const Product<T>& a)
 {
-    const long long tiles = a.tiles_p * a.tiles_q, groups = tiles * a.splits;
-    const long long per = (groups + NGS_XCDS - 1) / NGS_XCDS;
-    const long long t = (long long)(blockIdx.x % NGS_XCDS) * per + blockIdx.x / NGS_XCDS;
     Place w;
-    w.there = t < groups;
-    w.split = t / tiles;
-    const long long tile = t - w.split * tiles;
+    long long tile;
+    w.r_begin = 0;
+    w.r_end = a.nr;
+    w.partial = nullptr;
+    if (blockIdx.x < a.full_groups) {
+        tile = (long long)(blockIdx.x % NGS_XCDS) * (a.full_groups / NGS_XCDS) + blockIdx.x / NGS_XCDS;
+        w.there = tile < a.full;
+    } else {
+        const long long u = blockIdx.x - a.full_groups;
+        tile = a.full + u / a.parts;
+        w.there = true;
+        if (a.parts > 1) {
+            w.r_begin = u % a.parts * a.run;
+            w.r_end = w.r_begin + a.run < a.nr ? w.r_begin + a.run : a.nr;
+            w.partial = a.partial + u * (TP * TQ);
+        }
+    }
     w.p0 = (tile % a.tiles_p) * TP;
     w.q0 = (tile / a.tiles_p) * TQ;
-    w.r_begin = w.split * a.run;
-    w.r_end = w.r_begin + a.run < a.nr ? w.r_begin + a.run : a.nr;
     return w;
+}
+
+// A wave's share of a tile's sums, `first` elements into it
+template <int MP, int MQ, int TP>
+__device__ __forceinline__ void leave_partial(float* partial, const f32x4 (&acc)[MP][MQ], int p, int q, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < MP; i++)
+#pragma unroll
+        for (int j = 0; j < MQ; j++)
+            *(f32x4*)&partial[(q + j * 16 + (lane & 15)) * TP + p + i * 16 + (lane >> 4) * 4] = acc[i][j];
 }
 
 // A wave's MP x MQ fragments from (p0, q0) on: a lane holds four neighbouring p of one q.
 template <typename T, int MP, int MQ>
-__device__ __forceinline__ void finish_tile(const Product<T>& a, const f32x4 (&acc)[MP][MQ], long long p0, long long q0,
-                                            long long split, int lane)
+__device__ __forceinline__ void finish_tile(const Product<T>& a, const f32x4 (&acc)[MP][MQ], long long p0, long long q0, int lane)
 {
 #pragma unroll
     for (int i = 0; i < MP; i++) {
         const int p = (int)p0 + i * 16 + (lane >> 4) * 4;
         float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (p < a.np && a.epi.bias && !a.epi.partial) load4(a.epi.bias + p, bias, a.np - p);
+        if (p < a.np && a.epi.bias) load4(a.epi.bias + p, bias, a.np - p);
 #pragma unroll
         for (int j = 0; j < MQ; j++) {
             const long long q = q0 + j * 16 + (lane & 15);
-            if (p >= a.np || q >= a.nq) continue;
-            if (a.epi.partial) {
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                store4(a.epi.partial + (split * a.nq + q) * a.np + p, v, a.np - p);
-            } else {
-                finish4(a.epi, q, p, acc[i][j], bias);
-            }
+            if (p < a.np && q < a.nq) finish4(a.epi, q, p, acc[i][j], bias);
         }
     }
 }
@@ -92,7 +110,7 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_kernel(Product<T> a)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP, wq = wave / WP;
     const Place at = place_of<T, TP, TQ>(a);
     if (!at.there) return;
-    const long long p0 = at.p0, q0 = at.q0, r_begin = at.r_begin, r_end = at.r_end, split = at.split;
+    const long long p0 = at.p0, q0 = at.q0, r_begin = at.r_begin, r_end = at.r_end;
 
     f32x4 acc[MP][MQ];
 #pragma unroll
@@ -130,7 +148,8 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_kernel(Product<T> a)
         }
     }
 
-    finish_tile<T, MP, MQ>(a, acc, p0 + wp * MP * 16, q0 + wq * MQ * 16, split, lane);
+    if (at.partial) leave_partial<MP, MQ, TP>(at.partial, acc, wp * MP * 16, wq * MQ * 16, lane);
+    else finish_tile<T, MP, MQ>(a, acc, p0 + wp * MP * 16, q0 + wq * MQ * 16, lane);
 }
 
 // The same with operands that lie on 16-byte boundaries: they go from memory into shared memory without passing
@@ -206,23 +225,10 @@ constexpr int finish_wide_bytes() { return 16 * (MP * 16 + 4) * 4 + 16 * MP * 16
 
 template <typename T, int MP, int MQ, bool BARE>
 __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&acc)[MP][MQ], float* lds, long long p0,
-                                            long long q0, long long split, int lane)
+                                            long long q0, int lane)
 {
     constexpr int N = Chunk<T>::N, PITCH = MP * 16 + 4, LANES = MP * 16 / N, ROWS = 64 / LANES, TRIPS = 16 / ROWS;
     const int g = lane >> 4, i = lane & 15;
-    if (a.epi.partial) {
-#pragma unroll
-        for (int f = 0; f < MP; f++) {
-            const int p = (int)p0 + f * 16 + g * 4;
-#pragma unroll
-            for (int j = 0; j < MQ; j++) {
-                const long long q = q0 + j * 16 + i;
-                const float v[4] = {acc[f][j][0], acc[f][j][1], acc[f][j][2], acc[f][j][3]};
-                if (p < a.np && q < a.nq) store4(a.epi.partial + (split * a.nq + q) * a.np + p, v, a.np - p);
-            }
-        }
-        return;
-    }
     const int col = (lane % LANES) * N, p = (int)p0 + col, valid = a.np - p;
     float bias[N];
 #pragma unroll
@@ -338,32 +344,34 @@ __global__ __launch_bounds__(64 * WP * WQ) void product_direct_kernel(Product<T>
         }
         buf ^= 1;
     }
+    if (at.partial) {
+        leave_partial<MP, MQ, TP>(at.partial, acc, wp * MP * 16, wq * MQ * 16, lane);
+        return;
+    }
     __syncthreads();  // the tiles are done with
     static_assert(WAVES * finish_wide_bytes<T, MP>() <= 2 * STAGE, "a piece of the tiles' memory for each wave");
     finish_wide<T, MP, MQ, P_ACROSS>(a, acc, (float*)(lds + wave * finish_wide_bytes<T, MP>()), at.p0 + wp * MP * 16, at.q0 + wq * MQ * 16,
-                                     at.split, lane);
+                                     lane);
 }
 
-// Adds up the runs of a product that was cut along its reduction, in their order, and finishes it.
+// Adds up the parts of the tiles that several workgroups share, in their order, and finishes them.
 template <typename T>
-__global__ __launch_bounds__(256) void product_finish_kernel(const float* __restrict__ partial, int splits, long long nq,
-                                                             Epilogue<T> e)
+__global__ __launch_bounds__(256) void product_finish_kernel(const float* __restrict__ partial, int parts, long long full,
+                                                             long long tiles_p, int tp, int tq, long long nq, Epilogue<T> e)
 {
-    const long long per_row = (e.np + 3) / 4;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= per_row * nq) return;
-    const long long q = i / per_row;
-    const int p = (int)(i - q * per_row) * 4, valid = e.np - p;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < splits; s++) {
-        float v[4];
-        load4(partial + ((long long)s * nq + q) * e.np + p, v, valid);
-#pragma unroll
-        for (int k = 0; k < 4; k++) sum[k] += v[k];
-    }
+    const int quads = tp / 4 * tq, per = quads / 256;  // workgroups per tile
+    const long long shared = blockIdx.x / per, tile = full + shared;
+    const int i = (int)(blockIdx.x % per) * 256 + threadIdx.x, pt = i % (tp / 4) * 4, qt = i / (tp / 4);
+    const long long q = tile / tiles_p * tq + qt, p0 = tile % tiles_p * tp + pt;
+    if (p0 >= e.np || q >= nq) return;
+    const int p = (int)p0;
+    const float* at = partial + shared * parts * (tp * tq) + qt * tp + pt;
+    f32x4 sum = *(const f32x4*)at;
+#pragma unroll 4
+    for (int k = 1; k < parts; k++) sum += *(const f32x4*)(at + (long long)k * (tp * tq));
     float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (e.bias) load4(e.bias + p, bias, valid);
-    finish4(e, q, p, (f32x4){sum[0], sum[1], sum[2], sum[3]}, bias);
+    if (e.bias) load4(e.bias + p, bias, e.np - p);
+    finish4(e, q, p, sum, bias);
 }
 
 // ---------------------------------------------------------------------------
@@ -458,50 +466,76 @@ void ngs_launch_column_finish(hipStream_t s, const float* partial, long long blo
 // ---------------------------------------------------------------------------
 struct Shape {
     int tp, tq;
-    long long tiles_p, tiles_q;
-    int splits;
-    long long run;
-    static long long tiles(long long np, long long nq, long long t) { return ((np + t - 1) / t) * ((nq + t - 1) / t); }
-    long long groups() const { return (tiles_p * tiles_q * splits + NGS_XCDS - 1) / NGS_XCDS * NGS_XCDS; }
-    size_t partial_bytes(long long np, long long nq) const { return splits > 1 ? (size_t)splits * np * nq * 4 : 0; }
+    long long tiles_p, tiles_q, full, shared, run;  // as in Product; shared: tiles that `parts` workgroups share
+    int parts;
+    double cost;
+    long long full_groups() const { return (full + NGS_XCDS - 1) / NGS_XCDS * NGS_XCDS; }
+    size_t partial_bytes() const { return parts > 1 ? (size_t)shared * parts * tp * tq * 4 : 0; }
 };
 
 static inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Through registers, tiles are 128 wide unless the matrix is 32 or narrower; a reduction is cut until the tiles and its
-// runs fill the chip twice, each run at least four steps long.
-// Directly, tiles of 16-bit types are 256 x 256, one to a compute unit, or 128 x 128, two at a time.  A round of the
-// former takes one and a half times as long as one of the latter (8192 x 4096 -> 4096 bfloat16: 2 rounds 233 us, 4 rounds
-// 317 us; 6144 x 1024 -> 3200: 2 rounds 64 us, 2.3 rounds 51 us; 4096 x 1024 -> 2048: 35 us and 24 us, one round each); a
-// last round of small tiles that does not fill the chip costs about 0.6 of a full one.
-static Shape product_shape(long long np, long long nq, long long nr, int dtype, bool direct)
+// Microseconds that `count` workgroups take for a step of their reductions, side by side on the chip, as measured
+// (8192 x 4096 -> 4096 bfloat16, 64 steps: 2 rounds of 256 x 256 tiles 233 us, 4 rounds of 512 tiles of 128 x 128 317 us;
+// 2048 x 2048 -> 2048, 32 steps: 256 tiles of 128 x 128 30 us; float32, where the matrix units bound any tile:
+// 8192 x 4096 -> 4096, 128 steps: 2048 tiles of 128 x 128 2020 us).  Through registers, where what is large comes from rows
+// that start off a word's boundary, about four times as long (801 x 5556, 801 x 269 -> 5556 x 269 bfloat16: 62 us for 13 steps).
+static double step_us(int tp, int tq, long long count, int dtype, bool direct)
+{
+    const double rounds = (double)((count + NGS_CUS - 1) / NGS_CUS), area = (double)tp * tq / (128.0 * 128.0);
+    if (dtype == NGS_FLOAT32) {
+        const double busy = rounds * area * (direct ? 1.9 : 2.5);
+        return count > 0 && busy < 0.8 ? 0.8 : busy;
+    }
+    if (tp == 256) return rounds * 1.9;
+    const double whole = (double)(count / (2 * NGS_CUS));
+    const long long rest = count % (2 * NGS_CUS);
+    return (direct ? 1.0 : 4.0) * (1.25 * whole + (rest == 0 ? 0.0 : rest <= NGS_CUS ? 0.8 : 1.25)) * (area < 0.3 ? 0.6 : 1.0);
+}
+
+// Tiles of tp x tq, `slots` of which the chip works on at a time.  Rounds that fill it are computed whole.  The tiles of
+// the last round may share the chip: each is cut along the reduction into parts of at least four steps, and a second
+// kernel adds the parts up, which takes a launch and a way to memory and back.  5114 x 2776 -> 3400 bfloat16: 1080
+// tiles of 128 x 128 on 512 slots, 146 us in whole tiles, 114 us with the last 56 shared.
+static Shape shape_of(int tp, int tq, long long slots, long long np, long long nq, long long nr, int dtype, bool direct)
 {
     Shape s;
-    s.tp = np <= 32 ? 32 : 128;
-    s.tq = nq <= 32 ? 32 : 128;
-    if (direct && dtype == NGS_FLOAT32) {
-        // the matrix units bound either tile: the small one shares the work out more evenly
-        if (s.tiles(np, nq, 128) < 4 * NGS_CUS) s.tp = s.tq = 64;
-    } else if (direct) {
-        const long long large = ((np + 255) / 256) * ((nq + 255) / 256), small = ((np + 127) / 128) * ((nq + 127) / 128);
-        const double large_cost = 1.5 * (double)((large + NGS_CUS - 1) / NGS_CUS);
-        const double small_cost = (double)(small / (2 * NGS_CUS)) + (small % (2 * NGS_CUS) ? 0.6 : 0.0);
-        if (large_cost < small_cost) s.tp = s.tq = 256;
-    }
-    s.tiles_p = (np + s.tp - 1) / s.tp;
-    s.tiles_q = (nq + s.tq - 1) / s.tq;
+    s.tp = tp;
+    s.tq = tq;
+    s.tiles_p = (np + tp - 1) / tp;
+    s.tiles_q = (nq + tq - 1) / tq;
     const long long step = ROW_BYTES / (long long)ngs_decoder_size(dtype), steps = (nr + step - 1) / step;
-    const long long tiles = s.tiles_p * s.tiles_q;
-    long long cut = 1;
-    if (tiles > 0 && tiles < NGS_CUS && s.tp < 256) {
-        cut = (2 * NGS_CUS + tiles - 1) / tiles;
-        if (cut > steps / 4) cut = steps / 4;
-        if (cut < 1) cut = 1;
+    const long long tiles = s.tiles_p * s.tiles_q, last = tiles % slots;
+    s.parts = 1;
+    s.run = steps * step;
+    s.full = tiles;
+    s.cost = (double)steps * step_us(tp, tq, tiles, dtype, direct);
+    const long long most = last > 0 ? (slots / last < steps / 4 ? slots / last : steps / 4) : 1;
+    const double whole = (double)steps * step_us(tp, tq, tiles - last, dtype, direct);
+    for (long long p = 2; p <= most; p = p < most && p + (p + 1) / 2 > most ? most : p + (p + 1) / 2) {
+        const long long run = (steps + p - 1) / p, parts = (steps + run - 1) / run;
+        const double bytes = 2.0 * 4.0 * (double)(last * parts) * tp * tq;
+        const double cost = whole + (double)run * step_us(tp, tq, last * parts, dtype, direct) + 4.0 + bytes / 5.0e6;
+        if (cost < s.cost) {
+            s.cost = cost;
+            s.parts = (int)parts;
+            s.run = run * step;
+            s.full = tiles - last;
+        }
     }
-    const long long run = cut > 1 ? (steps + cut - 1) / cut : (steps > 0 ? steps : 1);
-    s.run = run * step;
-    s.splits = steps > 0 ? (int)((steps + run - 1) / run) : 1;
+    s.shared = tiles - s.full;
     return s;
+}
+
+// Through registers, tiles are 128 wide unless the matrix is 32 or narrower; directly, 128 x 128 or, of 16-bit types,
+// 256 x 256, or, of float32, 64 x 64, whichever should take less time.
+static Shape product_shape(long long np, long long nq, long long nr, int dtype, bool direct)
+{
+    if (!direct) return shape_of(np <= 32 ? 32 : 128, nq <= 32 ? 32 : 128, 2 * NGS_CUS, np, nq, nr, dtype, false);
+    const Shape a = shape_of(128, 128, 2 * NGS_CUS, np, nq, nr, dtype, true);
+    const Shape b = dtype == NGS_FLOAT32 ? shape_of(64, 64, 2 * NGS_CUS, np, nq, nr, dtype, true)
+                                         : shape_of(256, 256, NGS_CUS, np, nq, nr, dtype, true);
+    return b.cost < a.cost ? b : a;
 }
 
 // Whether product_direct_kernel has a tile for these sizes
@@ -524,7 +558,7 @@ static long long whole_chunks(long long width, int dtype)
 static bool pads(long long width, long long np, long long nq, long long nr, int dtype)
 {
     return width != whole_chunks(width, dtype) && direct_sizes(np, nq) &&
-           (double)np * (double)nq * (double)nr >= (dtype == NGS_FLOAT32 ? 268435456.0 : 2147483648.0);
+           (double)np * (double)nq * (double)nr >= (dtype == NGS_FLOAT32 ? 268435456.0 : 536870912.0);
 }
 
 // (rows2 rows of a second matrix of the same width follow the first's)
@@ -554,9 +588,9 @@ static void pad_rows(hipStream_t st, const T* from, long long ld, long long rows
 
 static size_t partial_bytes(long long np, long long nq, long long nr, int dtype)
 {
-    const size_t a = product_shape(np, nq, nr, dtype, false).partial_bytes(np, nq);
+    const size_t a = product_shape(np, nq, nr, dtype, false).partial_bytes();
     if (!direct_sizes(np, nq)) return a;
-    const size_t b = product_shape(np, nq, nr, dtype, true).partial_bytes(np, nq);
+    const size_t b = product_shape(np, nq, nr, dtype, true).partial_bytes();
     return a > b ? a : b;
 }
 
@@ -568,12 +602,15 @@ static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partia
     const Shape s = product_shape(a.np, a.nq, a.nr, dtype, direct);
     a.tiles_p = s.tiles_p;
     a.tiles_q = s.tiles_q;
-    a.splits = s.splits;
+    a.full = s.full;
+    a.full_groups = s.full_groups();
+    a.parts = s.parts;
     a.run = s.run;
+    a.partial = partial;
     a.epi.np = a.np;
-    a.epi.partial = s.splits > 1 ? partial : nullptr;
-    if (s.groups() > 0x7fffffffLL) return ngs_set_error("ngs_linear", "too many rows");
-    const dim3 grid((unsigned)s.groups());
+    const long long groups = a.full_groups + s.shared * s.parts;
+    if (groups > 0x7fffffffLL) return ngs_set_error("ngs_linear", "too many rows");
+    const dim3 grid((unsigned)groups);
     if (direct && s.tp == 128) {
         hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
     } else if (direct) {
@@ -590,11 +627,10 @@ static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partia
     } else {
         hipLaunchKernelGGL((product_kernel<T, PA, QA, 32, 32, 2, 2>), grid, dim3(256), 0, st, a);
     }
-    if (s.splits > 1) {
-        Epilogue<T> e = a.epi;
-        const long long items = (a.np + 3LL) / 4 * a.nq;
-        hipLaunchKernelGGL(product_finish_kernel<T>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, partial,
-                           s.splits, a.nq, e);
+    if (s.parts > 1) {
+        const long long finish = s.shared * (s.tp * s.tq / 1024);
+        hipLaunchKernelGGL(product_finish_kernel<T>, dim3((unsigned)finish), dim3(256), 0, st, partial, s.parts, s.full,
+                           s.tiles_p, s.tp, s.tq, a.nq, a.epi);
     }
     return ngs_decoder_launched("ngs_linear");
 }

@@ -93,7 +93,6 @@ struct Epilogue {
     long long ldr;
     T* y;                 // [nq][np]
     typename Slope<T>::type* slope;  // [nq][np] or NULL
-    float* partial;       // not NULL: the bare sums go to partial[split][q][p] and nothing else happens
 };
 
 template <typename U>

@@ -56,7 +56,7 @@ def check_linear(ops, rows, k, n, dtype, act, bias, residual, train=True, first=
 
 LINEAR_SIZES = [(1, 1, 1), (1, 64, 128), (3, 39, 3), (5, 17, 31), (16, 8, 40), (33, 100, 65), (127, 128, 129),
                 (128, 64, 128), (130, 200, 300), (257, 513, 40), (1000, 39, 3), (300, 1030, 520), (4100, 24, 16),
-                (2, 4096, 1000), (64, 5000, 48), (7, 3, 700), (40, 2050, 33), (2600, 128, 128), (2049, 64, 96), (8192, 64, 1024), (3000, 1000, 1000), (2048, 264, 3400), (600, 4104, 600), (2300, 1001, 1003), (1500, 1203, 1208), (1500, 1208, 1203),
+                (2, 4096, 1000), (64, 5000, 48), (7, 3, 700), (40, 2050, 33), (2600, 128, 128), (2049, 64, 96), (8192, 64, 1024), (3000, 1000, 1000), (2048, 264, 3400), (600, 4104, 600), (2300, 1001, 1003), (1500, 1203, 1208), (1500, 1208, 1203), (8200, 304, 2000), (4099, 1001, 2003),
                 (515, 256, 256), (9, 1027, 2051), (12, 512, 512), (1, 8192, 70), (4, 1111, 999), (8, 2048, 3), (15, 640, 4097), (16, 33, 5), (17, 700, 64), (33, 1001, 50), (64, 3711, 40), (60, 9, 17),
                 # many narrow rows
                 (4096, 1, 1), (4097, 3, 5), (5000, 39, 3), (4999, 128, 128), (4100, 127, 129), (6001, 200, 24), (4200, 17, 100),
