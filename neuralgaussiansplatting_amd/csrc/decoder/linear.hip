@@ -426,21 +426,26 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long rows, int n, i
     }
 }
 
-// 16 columns by 64 rows of threads: a thread adds every 64th row, the 64 sums are joined pairwise.
-template <typename T>
+// COLS columns by 1024 / COLS rows of threads: a thread adds every so many rows, the threads' sums are joined pairwise.
+// Sixteen columns spread a few columns over many threads; 64 read whole lines, where there are enough of them to fill
+// the chip (512 x 10002: 12 us by 16, DRAM lines read in quarters).
+template <typename T, int COLS>
 __global__ __launch_bounds__(1024) void column_finish_kernel(const float* __restrict__ partial, long long blocks,
                                                              long long width0, long long width1, T* __restrict__ out0,
                                                              T* __restrict__ out1)
 {
-    __shared__ float sums[64][17];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const long long c = (long long)blockIdx.x * 16 + tx, pitch = width0 + width1;
+    constexpr int ROWS = 1024 / COLS;
+    __shared__ float sums[ROWS][COLS + 1];
+    const int tx = threadIdx.x % COLS, ty = threadIdx.x / COLS;
+    const long long c = (long long)blockIdx.x * COLS + tx, pitch = width0 + width1;
     float s = 0.0f;
-    if (c < pitch)
-        for (long long b = ty; b < blocks; b += 64) s += partial[b * pitch + c];
+    if (c < pitch) {
+#pragma unroll 8
+        for (long long b = ty; b < blocks; b += ROWS) s += partial[b * pitch + c];
+    }
     sums[ty][tx] = s;
     __syncthreads();
-    for (int half = 32; half > 0; half >>= 1) {
+    for (int half = ROWS / 2; half > 0; half >>= 1) {
         if (ty < half) sums[ty][tx] += sums[ty + half][tx];
         __syncthreads();
     }
@@ -449,16 +454,25 @@ __global__ __launch_bounds__(1024) void column_finish_kernel(const float* __rest
     if (out) out[c < width0 ? c : c - width0] = (T)sums[0][tx];
 }
 
+template <typename T>
+static void column_finish(hipStream_t s, const float* partial, long long blocks, long long width0, long long width1, void* out0,
+                          void* out1)
+{
+    const long long pitch = width0 + width1;
+    if (pitch >= 32 * NGS_CUS)
+        hipLaunchKernelGGL((column_finish_kernel<T, 64>), dim3((unsigned)((pitch + 63) / 64)), dim3(1024), 0, s, partial, blocks,
+                           width0, width1, (T*)out0, (T*)out1);
+    else
+        hipLaunchKernelGGL((column_finish_kernel<T, 16>), dim3((unsigned)((pitch + 15) / 16)), dim3(1024), 0, s, partial, blocks,
+                           width0, width1, (T*)out0, (T*)out1);
+}
+
 void ngs_launch_column_finish(hipStream_t s, const float* partial, long long blocks, long long width0, long long width1,
                               void* out0, void* out1, int dtype)
 {
-    const dim3 grid((unsigned)((width0 + width1 + 15) / 16)), threads(1024);
-    if (dtype == NGS_FLOAT32)
-        hipLaunchKernelGGL(column_finish_kernel<float>, grid, threads, 0, s, partial, blocks, width0, width1, (float*)out0, (float*)out1);
-    else if (dtype == NGS_FLOAT16)
-        hipLaunchKernelGGL(column_finish_kernel<f16>, grid, threads, 0, s, partial, blocks, width0, width1, (f16*)out0, (f16*)out1);
-    else
-        hipLaunchKernelGGL(column_finish_kernel<bf16>, grid, threads, 0, s, partial, blocks, width0, width1, (bf16*)out0, (bf16*)out1);
+    if (dtype == NGS_FLOAT32) column_finish<float>(s, partial, blocks, width0, width1, out0, out1);
+    else if (dtype == NGS_FLOAT16) column_finish<f16>(s, partial, blocks, width0, width1, out0, out1);
+    else column_finish<bf16>(s, partial, blocks, width0, width1, out0, out1);
 }
 
 // ---------------------------------------------------------------------------
