@@ -7,7 +7,8 @@ _CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 
 
 def kernel_sources_sha():
-    """First 16 hex digits of the SHA-256 over the HIP sources and headers of the library, in name order."""
+    """First 16 hex digits of the SHA-256 over the HIP sources and headers of the rasterizer, in name order (the kept
+    counters are of its kernels; the operators over feature rows, in csrc/decoder, share none of them)."""
     h = hashlib.sha256()
     for name in sorted(os.listdir(_CSRC)):
         if name.endswith((".hip", ".h")):

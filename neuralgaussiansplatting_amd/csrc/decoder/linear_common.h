@@ -9,8 +9,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 #define ROW_BYTES 128  // bytes of the reduction index that one step stages per row: 64 16-bit elements or 32 floats
 
-#define NGS_STREAM_ROWS 4096
-#define NGS_FEW_ROWS 64
+#define NGS_FEW_ROWS 64  // rows that linear_rows.hip takes at most
 
 // Elements of the derivative array for T.
 template <typename T> struct Slope { typedef f16 type; };

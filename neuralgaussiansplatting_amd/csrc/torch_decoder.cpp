@@ -89,9 +89,9 @@ hipStream_t stream_of(const Tensor& t)
 
 Tensor workspace_of(const Tensor& x, size_t bytes)
 {
-    return torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8).requires_grad(false));
+    return bytes ? torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8).requires_grad(false)) : Tensor();
 }
-char* bytes_ptr(Tensor& t) { return t.numel() ? reinterpret_cast<char*>(t.data_ptr()) : nullptr; }
+char* bytes_ptr(Tensor& t) { return t.defined() ? reinterpret_cast<char*>(t.data_ptr()) : nullptr; }
 
 std::vector<int64_t> with_last(const Tensor& x, int64_t last)
 {
@@ -114,7 +114,11 @@ void check_capture(const char* what, const c10::optional<Tensor>& t)
     if (!wants_grad(t) || !t->is_leaf()) return;
     const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t->device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {
+        (void)hipGetLastError();  // not this call's failure to report
+        return;
+    }
+    if (status == hipStreamCaptureStatusNone) return;
     const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
     if (!accumulator) return;
     const auto its = accumulator->stream();
