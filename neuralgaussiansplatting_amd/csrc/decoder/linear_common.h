@@ -30,8 +30,8 @@ __device__ __forceinline__ float activate_one(float z, float& slope)
     if (ACT == NGS_ACT_GELU) {
         // Phi by the rational approximation 7.1.26 of Abramowitz and Stegun's handbook (erfc x = P(t) exp(-x^2),
         // t = 1 / (1 + 0.3275911 x), error below 1.5e-7, halved here): its exponential is the density's, which the
-        // derivative needs.  About 20 issue slots; erff and an exponential of its own take three times as many, which
-        // bounded the narrow products (640000 x 128 -> 128 bfloat16: 162 us forward, against 492 MB to move).
+        // derivative needs.  The narrow products feel the difference (640000 x 128 -> 128 bfloat16 with residual: forward
+        // 110 us, there and back 268 us; 122 us and 329 us with erff and an exponential of its own, all else alike).
         const float e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
         const float t = __builtin_amdgcn_rcpf(1.0f + 0.23164188f * fabsf(z));
         const float tail = 0.5f * e * (t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f +
