@@ -412,7 +412,8 @@ int ngs_idxmap_forward_static(int P, int width, int height, const float* means3D
  *
  * dtype names the element type of every array typed void* unless noted.  Row strides are in elements and may be any
  * non-negative number; elements of a row are contiguous, and so are outputs, rows included.  Arrays need the
- * alignment of their element type only; a workspace needs 16 bytes.  Sums, statistics and activations are formed in
+ * alignment of their element type only; a workspace needs 16 bytes.  Rows of linear and layer norm have at most 2^30 elements; what
+ * a launch does not hold is refused.  Sums, statistics and activations are formed in
  * 32 bits, each output is rounded once, and results do not depend on timing (no atomics).  Sizes of zero are fine.
  * Outputs must not overlap inputs, unless noted.
  *

@@ -104,6 +104,14 @@ inline int ngs_decoder_launched(const char* what)
     return e == hipSuccess ? 0 : ngs_set_error(what, hipGetErrorString(e));
 }
 
+#define NGS_WIDEST (1 << 30)  // columns of a row at most: kernels count them, a tile past the end, in 32 bits
+
+// A launch has fewer than 2^32 threads along x.
+inline int ngs_decoder_grid(const char* what, long long groups, int threads)
+{
+    return groups > 0xffffffffLL / threads ? ngs_set_error(what, "too many elements for one launch") : 0;
+}
+
 inline bool ngs_decoder_dtype(int t) { return t == NGS_FLOAT32 || t == NGS_FLOAT16 || t == NGS_BFLOAT16; }
 inline size_t ngs_decoder_size(int t) { return t == NGS_FLOAT32 ? 4 : 2; }
 

@@ -105,7 +105,7 @@ static int run_dropout(hipStream_t st, DropoutArgs<T> a)
         a.rows = 1;
     }
     const long long groups = ((a.total + 7) / 8 + 255) / 256;
-    if (groups > 0x7fffffffLL) return ngs_set_error("ngs_dropout", "too many elements");
+    if (ngs_decoder_grid("ngs_dropout", groups, 256)) return 1;
     hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)groups), dim3(256), 0, st, a);
     return ngs_decoder_launched("ngs_dropout");
 }

@@ -405,8 +405,8 @@ static NormShape norm_shape(long long width, int dtype)
     if (c <= 1536) return G512x3;
     if (c <= 2048) return G512x4;
     // (16-bit types hold twice as many elements per chunk: no registers for more)
-    if (dtype == NGS_FLOAT32 && c <= 3072) return G1024x3;
-    if (dtype == NGS_FLOAT32 && c <= 4096) return G1024x4;
+    if (dtype == NGS_FLOAT32 && c <= 3 * 1024) return G1024x3;
+    if (dtype == NGS_FLOAT32 && c <= 4 * 1024) return G1024x4;
     return NORM_WIDE;
 }
 
@@ -452,7 +452,7 @@ static int norm_forward(hipStream_t st, int dtype, NormArgs<T, W> a)
 {
     const NormShape s = norm_shape(a.width, dtype);
     if (s == NORM_WIDE) {
-        if (a.rows > 0x7fffffffLL) return ngs_set_error("ngs_layer_norm_forward", "too many rows");
+        if (ngs_decoder_grid("ngs_layer_norm_forward", a.rows, 1024)) return 1;
         hipLaunchKernelGGL((norm_forward_wide_kernel<T, W>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
         return ngs_decoder_launched("ngs_layer_norm_forward");
     }
@@ -469,7 +469,7 @@ static int norm_backward(hipStream_t st, int dtype, int weight_dtype, NormBackwa
 {
     const unsigned blocks = (unsigned)norm_backward_blocks(a.rows, a.width, dtype);
     if (norm_shape(a.width, dtype) == NORM_WIDE) {
-        if (a.rows > 0x7fffffffLL) return ngs_set_error("ngs_layer_norm_backward", "too many rows");
+        if (ngs_decoder_grid("ngs_layer_norm_backward", a.rows, 1024)) return 1;
         if (a.dx)
             hipLaunchKernelGGL((norm_backward_wide_kernel<T, W>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
         if (a.partial) {
@@ -488,7 +488,8 @@ static int norm_backward(hipStream_t st, int dtype, int weight_dtype, NormBackwa
 static int check_norm(const char* what, long long rows, int width, int dtype, int weight_dtype)
 {
     if (rows < 0 || width < 0) return ngs_set_error(what, "a size is negative");
-    if (rows > (1LL << 40) || (double)rows * width > 281474976710656.0) return ngs_set_error(what, "too many elements");
+    if (rows > (1LL << 40) || width > NGS_WIDEST || (double)rows * width > 281474976710656.0)
+        return ngs_set_error(what, "too many elements for one launch");
     if (!ngs_decoder_dtype(dtype) || !ngs_decoder_dtype(weight_dtype)) return ngs_set_error(what, "unknown element type");
     if (weight_dtype != dtype && weight_dtype != NGS_FLOAT32)
         return ngs_set_error(what, "the weights must be of the rows' type or float32");

@@ -627,7 +627,7 @@ static int launch_product(hipStream_t st, int dtype, Product<T> a, float* partia
     a.partial = partial;
     a.epi.np = a.np;
     const long long groups = a.full_groups + s.shared * s.parts;
-    if (groups > 0x7fffffffLL) return ngs_set_error("ngs_linear", "too many rows");
+    if (ngs_decoder_grid("ngs_linear", groups, direct && s.tp == 256 ? 512 : 256)) return 1;
     const dim3 grid((unsigned)groups);
     if (direct && s.tp == 128) {
         hipLaunchKernelGGL((product_direct_kernel<T, PA, QA, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
@@ -801,13 +801,13 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
 // (byte counts of operands and workspaces stay far from 64 bits)
 static bool too_many(long long rows, int k, int n)
 {
-    return rows > (1LL << 40) || (double)rows * (k > n ? k : n) > 281474976710656.0;
+    return rows > (1LL << 40) || k > NGS_WIDEST || n > NGS_WIDEST || (double)rows * (k > n ? k : n) > 281474976710656.0;
 }
 
 static int check_linear(const char* what, long long rows, int k, int n, int dtype, int act)
 {
     if (rows < 0 || k < 0 || n < 0) return ngs_set_error(what, "a size is negative");
-    if (too_many(rows, k, n)) return ngs_set_error(what, "too many elements");
+    if (too_many(rows, k, n)) return ngs_set_error(what, "too many elements for one launch");
     if (!ngs_decoder_dtype(dtype)) return ngs_set_error(what, "unknown element type");
     if (act < NGS_ACT_NONE || act > NGS_ACT_SIGMOID) return ngs_set_error(what, "unknown activation");
     return 0;

@@ -93,6 +93,7 @@ static int few_rows_launch(hipStream_t st, FewRows<T> a)
     // waves: until the chip holds 16 to a compute unit, while each has four steps
     int waves = 1;
     while (waves < 16 && (long long)groups * waves < 16 * NGS_CUS && steps >= 8 * waves) waves *= 2;
+    if (ngs_decoder_grid("ngs_linear_forward", groups, 64 * waves)) return 1;
     a.run = (steps + waves - 1) / waves;
     const size_t lds = waves > 1 ? (size_t)waves * QF * 64 * sizeof(f32x4) : 0;
     const bool any = sizeof(T) == 2 && (((uintptr_t)a.x | (uintptr_t)a.w) & 3 || (a.ldx | a.ldw) & 1);

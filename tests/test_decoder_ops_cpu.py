@@ -68,6 +68,17 @@ def test_c_entries_refuse(lib, case):
     assert lib.ngs_last_error()
 
 
+@pytest.mark.parametrize("call,args", [
+    (linear, dict(rows=1 << 31, k=300, n=32, ldx=0, ldw=300)), (linear, dict(k=8, n=(1 << 31) - 1)),
+    (linear, dict(k=(1 << 31) - 1)),
+    (linear_backward, dict(n=(1 << 31) - 1)), (norm, dict(d=(1 << 31) - 1)), (norm, dict(rows=1 << 23, d=20000, ldx=0)), (dropout, dict(rows=1, d=1 << 36, ldx=0)),
+])
+def test_c_entries_refuse_what_one_launch_does_not_hold(lib, call, args):
+    assert call(lib, **args) != 0
+    lib.ngs_last_error.restype = ctypes.c_char_p
+    assert b"too many elements for one launch" in lib.ngs_last_error()
+
+
 def test_c_entries_with_nothing_to_do(lib):
     """Sizes of zero return without touching an address (or a GPU)."""
     assert linear(lib, rows=0, x=None, y=None, ws=None) == 0
