@@ -62,14 +62,16 @@ void check_like(const char* what, const char* name, const Tensor& t, const Tenso
 }
 
 // A tensor as rows of `width` elements that follow each other at a fixed stride; a copy where its strides do not allow
-// that (elements of a row not contiguous, leading dimensions that do not collapse).
+// that (elements of a row not contiguous, leading dimensions that do not collapse) or where its memory holds the
+// negated values (torch's lazy negation).
 struct Rows {
     Tensor t;
     int64_t rows, width, stride;
 };
 
-Rows rows_of(const Tensor& x, int64_t width)
+Rows rows_of(const Tensor& given, int64_t width)
 {
+    const Tensor x = given.is_neg() ? given.resolve_neg() : given;
     int64_t rows = 1;
     for (int64_t d = 0; d + 1 < x.dim(); d++) rows *= x.size(d);
     Tensor t = x.dim() == 2 ? x : x.reshape({rows, width});
@@ -77,7 +79,7 @@ Rows rows_of(const Tensor& x, int64_t width)
     return {t, rows, width, t.stride(0)};
 }
 
-Tensor vec(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+Tensor vec(const Tensor& t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.is_contiguous() ? t : t.contiguous(); }
 
 const void* ptr(const c10::optional<Tensor>& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
 bool wants_grad(const c10::optional<Tensor>& t) { return t.has_value() && t->defined() && t->requires_grad(); }

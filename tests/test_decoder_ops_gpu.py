@@ -633,3 +633,25 @@ def _kept_from(first, count, p, seed):
             k0, k1 = (k0 + 0x9E3779B9) & word, (k1 + 0xBB67AE85) & word
         out += [(v >> s & 0xFFFF) >= round(p * 65536) for v in (a, b, c, d) for s in (0, 16)]
     return out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lazily_negated_tensors(ops, dtype):
+    """A view whose memory holds the negated values counts as its values: the same bits as from a plain copy."""
+    g = gen(12)
+
+    def pair(*shape):
+        lazy = torch._neg_view(normal(g, *shape, dtype=dtype))
+        assert lazy.is_neg()
+        return lazy, lazy.clone().resolve_neg()
+
+    (x, px), (w, pw), (b, pb), (r, pr), (dy, pdy) = pair(200, 40), pair(24, 40), pair(24), pair(200, 24), pair(200, 24)
+    (v, pv), (c, pc) = pair(40), pair(40)
+    calls = [lambda x, w, b, r, v, c: ops.linear(x, w, b, activation="gelu", residual=r),
+             lambda x, w, b, r, v, c: ops.layer_norm(x, v, c) @ torch.ones(40, 24, device=DEV, dtype=dtype),
+             lambda x, w, b, r, v, c: ops.dropout(x, 0.3, 5)[:, :24] + r]
+    for call in calls:
+        assert torch.equal(call(x, w, b, r, v, c), call(px, pw, pb, pr, pv, pc))
+    leaf = px.clone().requires_grad_(True)
+    lazy, plain = (torch.autograd.grad(ops.linear(leaf, pw, pb, activation="silu"), leaf, d)[0] for d in (dy, pdy))
+    assert torch.equal(lazy, plain)
