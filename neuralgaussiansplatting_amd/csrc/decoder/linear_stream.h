@@ -16,7 +16,7 @@
 // large copy's rate), backward 492 MB in 195 us (2.5 TB/s).  Without an activation the two together take 211 us instead
 // of 268 us, so forming z and the derivative again is about 40 us of the backward pass; 242 registers a lane leave it two
 // waves to a SIMD, too few to hide the rest under the loads.  1920 x 1080 rows 64 -> 128 float32 forward with relu moves
-// 1.59 GB in 364 us (4.4 TB/s).
+// 1.59 GB in 359 us (4.4 TB/s).
 #pragma once
 #include "linear_common.h"
 
