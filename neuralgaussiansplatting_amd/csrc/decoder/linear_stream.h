@@ -12,11 +12,11 @@
 // weight (dx) and, with x, through shared memory into the product over the rows (dW), whose sums stay in registers
 // until the workgroup is done.
 //
-// Measured: 640000 rows 128 -> 128 bfloat16 with gelu and residual, kernel times: forward 492 MB in 100 us (4.9 TB/s, at a
-// large copy's rate), backward 492 MB in 195 us (2.5 TB/s).  Without an activation the two together take 211 us instead
+// Measured: 640000 rows 128 -> 128 bfloat16 with gelu and residual, kernel times: forward 492 MB in 99 us (5.0 TB/s, at a
+// large copy's rate), backward 492 MB in 193 us (2.5 TB/s).  Without an activation the two together take 211 us instead
 // of 268 us, so forming z and the derivative again is about 40 us of the backward pass; 242 registers a lane leave it two
 // waves to a SIMD, too few to hide the rest under the loads.  1920 x 1080 rows 64 -> 128 float32 forward with relu moves
-// 1.59 GB in 359 us (4.4 TB/s).
+// 1.59 GB in 357 us (4.5 TB/s).
 #pragma once
 #include "linear_common.h"
 
@@ -258,6 +258,26 @@ __global__ __launch_bounds__(THREADS) void stream_forward_kernel(StreamForward<T
 // ---------------------------------------------------------------------------
 // Backward
 // ---------------------------------------------------------------------------
+// Backward: the product of x's and dz's steps that one workgroup's shared memory holds (the weight, and the tiles of 16
+// rows per wave).
+constexpr int stream_most(int size) { return size == 4 ? 64 : 32; }
+// Waves of a workgroup: eight share a large weight; four where a wave holds more than 256 registers' worth, and where
+// little enough is held that several workgroups fit a compute unit and need not wait together (640000 rows 39 -> 3
+// float32 there and back: 153 us by eights, 134 us by fours, with a grid of four to a unit).
+constexpr int stream_waves(int ks, int ns, int size)
+{
+    return ks * ns <= 8 || ks * ns > 32 || ks > 8 || ns > 8 || (size == 2 && (ks > 4 || ns > 4)) ? 4 : 8;
+}
+// Workgroups of a compute unit: what its registers hold, which is asked of the compiler as well, so that the launch is one
+// round and no unit works on a second while others wait (640000 rows 39 (of 64) -> 3 float32 there and back: 116 us, 133 us
+// with four workgroups where three were held; 200 -> 3 bfloat16 190 us, 278 us).
+constexpr int stream_per_cu(int ks, int ns, int size)
+{
+    if (stream_waves(ks, ns, size) == 8) return 1;
+    if (size == 4) return ks * ns <= 4 ? 4 : ks * ns <= 8 ? (ks <= 4 && ns <= 4 ? 3 : 2) : 1;
+    return ks * ns <= 2 ? 4 : ks * ns <= 4 && ns <= 2 ? 3 : ks * ns <= 8 && ns <= 4 ? 2 : 1;
+}
+
 template <typename T>
 struct StreamBackward {
     long long rows, tiles;
@@ -271,10 +291,10 @@ struct StreamBackward {
 };
 
 // KS, NS: steps of four chunks that a row of x and of dz take; SHORT_X, SHORT_Z: they are shorter than
-// a chunk.  As in the
-// forward pass, dx is kept until the next rows have arrived, where there are registers for it.
+// a chunk.  As in the forward pass, dx is kept until the next rows have arrived, where there are registers for it.
 template <typename T, int KS, int NS, bool SHORT_X, bool SHORT_Z, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void stream_backward_kernel(StreamBackward<T> a)
+__global__ __launch_bounds__(64 * WAVES, stream_per_cu(KS, NS, sizeof(T)) * (WAVES / 4))
+void stream_backward_kernel(StreamBackward<T> a)
 {
     constexpr int N = Chunk<T>::N, CK = KS * 4, CN = NS * 4, PARTS = N / 4;
     constexpr int TK = CK * N, TN = CN * N, TM = WAVES * 16;          // columns of x, columns of dz, rows of a tile
@@ -505,17 +525,6 @@ inline int steps_of(long long width, int dtype)  // steps of four chunks, as a p
     return s;
 }
 
-// Backward: the product of x's and dz's steps that one workgroup's shared memory holds (the weight, and the tiles of 16
-// rows per wave).
-constexpr int stream_most(int size) { return size == 4 ? 64 : 32; }
-// Waves of a workgroup: eight share a large weight; four where a wave holds more than 256 registers' worth, and where
-// little enough is held that several workgroups fit a compute unit and need not wait together (640000 rows 39 -> 3
-// float32 there and back: 153 us by eights, 134 us by fours).
-constexpr int stream_waves(int ks, int ns, int size)
-{
-    return ks * ns <= 8 || ks * ns > 32 || ks > 8 || ns > 8 || (size == 2 && (ks > 4 || ns > 4)) ? 4 : 8;
-}
-
 // groups of four chunks of the result per workgroup: 1, 4 or 8
 inline int stream_blocks(int n, int dtype)
 {
@@ -528,8 +537,15 @@ static int stream_forward_launch(hipStream_t st, const StreamForward<T>& a)
 {
     constexpr int COLS = NB * 4 * Chunk<T>::N, LDS = COLS * (KS * 64 + 4);
     constexpr int THREADS = LDS > 32 * 1024 ? 512 : 256;
-    constexpr int PER_CU = 160 * 1024 / LDS < 2048 / THREADS ? 160 * 1024 / LDS : 2048 / THREADS;
-    const long long need = ((a.rows + 15) / 16 + THREADS / 64 - 1) / (THREADS / 64), most = NGS_CUS * PER_CU;
+    // Two rounds of what a compute unit holds at a time: a part of a round would leave units idle at the end, and with one
+    // round alone the slowest workgroup is waited for (2000000 rows 64 -> 3 bfloat16 with residual: 84 us; 97 us with eight
+    // to a unit, of which six are held; 32 -> 32: 75 us, 83 us with eight, 89 us with one round).
+    static const int held = [] {
+        int n = 0;
+        const void* const kernel = (const void*)stream_forward_kernel<T, KS, NB, SHORT, RESIDUAL, THREADS>;
+        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, THREADS, 0) == hipSuccess && n > 0 ? n : 4;
+    }();
+    const long long need = ((a.rows + 15) / 16 + THREADS / 64 - 1) / (THREADS / 64), most = 2LL * NGS_CUS * held;
     const dim3 grid((unsigned)(need < most ? need : most), (unsigned)((a.n + COLS - 1) / COLS));
     hipLaunchKernelGGL((stream_forward_kernel<T, KS, NB, SHORT, RESIDUAL, THREADS>), grid, dim3(THREADS), 0, st, a);
     return ngs_decoder_launched("ngs_linear_forward");

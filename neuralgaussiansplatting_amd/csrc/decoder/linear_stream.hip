@@ -10,26 +10,18 @@ bool ngs_stream_forward_takes(long long rows, int k, int n, int dtype)
     return steps_of(k, dtype) <= 8 && n <= 2 * 8 * 64 / (int)ngs_decoder_size(dtype);
 }
 
-static size_t stream_backward_lds(int ks, int ns, int size)
-{
-    const int tn = ns * 64 / size, tm = stream_waves(ks, ns, size) * 16;
-    return (size_t)tn * ks * 64 + (size_t)tm * (ks + ns) * 64 + tn * 4;
-}
-
 bool ngs_stream_backward_takes(long long rows, int k, int n, int dtype)
 {
     if (rows < 1 || k < 1 || n < 1) return false;
     const int size = (int)ngs_decoder_size(dtype), ks = steps_of(k, dtype), ns = steps_of(n, dtype);
     return ks <= 4 * size && ns <= 4 * size && ks * ns <= stream_most(size);  // a width of 256
-
 }
 
 long long ngs_stream_backward_blocks(long long rows, int k, int n, int dtype)
 {
     const int size = (int)ngs_decoder_size(dtype), ks = steps_of(k, dtype), ns = steps_of(n, dtype);
     const int tm = stream_waves(ks, ns, size) * 16;
-    const long long tiles = (rows + tm - 1) / tm, per_cu = (long long)(160 * 1024 / stream_backward_lds(ks, ns, size));
-    const long long most = NGS_CUS * (per_cu < 1 ? 1 : per_cu < 4 ? per_cu : 4);
+    const long long tiles = (rows + tm - 1) / tm, most = NGS_CUS * stream_per_cu(ks, ns, size);
     return tiles < most ? tiles : most;
 }
 
