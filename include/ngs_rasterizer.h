@@ -421,10 +421,9 @@ int ngs_idxmap_forward_static(int P, int width, int height, const float* means3D
  * [out_features][in_features] (rows weight_stride apart), bias [out_features] or NULL, residual [rows][out_features]
  * (rows residual_stride apart) or NULL, y [rows][out_features].  GELU is x Phi(x), SILU x sigmoid(x).  slope, if not
  * NULL, receives the activation's derivative at every element, [rows][out_features], for the backward pass: floats
- * for NGS_FLOAT32, half precision (NGS_FLOAT16) for both 16-bit types -- the derivative is bounded, so its 11 bits
- * are finer than the types' own rounding of the gradient.  NGS_ACT_NONE needs none and writes none.
- * ngs_linear_backward_reads_slope says whether the backward pass of these sizes reads it (1) or forms z again from x,
- * weight and bias (0: slope may be NULL in both calls).
+ * whatever the dtype (a saturated unit's derivative is smaller than what 16 bits hold).  NGS_ACT_NONE needs none and
+ * writes none.  ngs_linear_slope_bytes is the size of that array in bytes where the backward pass of these sizes reads
+ * it, and 0 where it forms z again from x, weight and bias (slope may be NULL in both calls then).
  *
  * ngs_linear_backward: with dz = dL_dy * slope, dL_dx = dz weight, dL_dweight = dz^T x, dL_dbias = sum of dz over the
  * rows; any of the three may be NULL.  bias as in the forward call.  dL_dy [rows][out_features], rows dL_dy_stride apart.  (A residual's gradient
@@ -459,14 +458,14 @@ int ngs_idxmap_forward_static(int P, int width, int height, const float* means3D
 size_t ngs_linear_forward_workspace_bytes(long long rows, int in_features, int out_features, int dtype);
 int ngs_linear_forward(long long rows, int in_features, int out_features, int dtype, int activation, const void* x,
                        long long x_stride, const void* weight, long long weight_stride, const void* bias,
-                       const void* residual, long long residual_stride, void* y, void* slope, char* workspace,
+                       const void* residual, long long residual_stride, void* y, float* slope, char* workspace,
                        void* stream);
-int ngs_linear_backward_reads_slope(long long rows, int in_features, int out_features, int dtype, int activation);
+size_t ngs_linear_slope_bytes(long long rows, int in_features, int out_features, int dtype, int activation);
 size_t ngs_linear_backward_workspace_bytes(long long rows, int in_features, int out_features, int dtype,
                                            int activation);
 int ngs_linear_backward(long long rows, int in_features, int out_features, int dtype, int activation, const void* x,
                         long long x_stride, const void* weight, long long weight_stride, const void* bias,
-                        const void* slope, const void* dL_dy, long long dL_dy_stride, void* dL_dx, void* dL_dweight,
+                        const float* slope, const void* dL_dy, long long dL_dy_stride, void* dL_dx, void* dL_dweight,
                         void* dL_dbias, char* workspace, void* stream);
 int ngs_layer_norm_forward(long long rows, int width, int dtype, int weight_dtype, float eps, const void* x,
                            long long x_stride, const void* weight, const void* bias, void* y, float* mean, float* rstd,

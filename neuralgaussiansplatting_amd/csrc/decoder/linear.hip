@@ -274,10 +274,12 @@ __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&a
             } else {
                 float slope[N];
                 if (a.epi.slope) {
-                    typedef typename Slope<T>::type S;
-                    static_assert(sizeof(S) == sizeof(T), "a chunk of derivatives beside a chunk of results");
                     activate<N>(a.epi.act, z, y, slope);
-                    store16_head(a.epi.slope + q * a.np + p, pack<S>(slope), valid);
+#pragma unroll
+                    for (int e = 0; e < N; e += 4) {
+                        const float four[4] = {slope[e], slope[e + 1], slope[e + 2], slope[e + 3]};
+                        if (e < valid) store4(a.epi.slope + q * a.np + p + e, four, valid - e);
+                    }
                 } else {
                     activate<N>(a.epi.act, z, y, nullptr);
                 }
@@ -384,7 +386,7 @@ __global__ __launch_bounds__(256) void product_finish_kernel(const float* __rest
 // 201 MB in 39 us (5.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(long long rows, int n, int across, const T* __restrict__ dy,
-                                                        long long lddy, const typename Slope<T>::type* __restrict__ slope,
+                                                        long long lddy, const float* __restrict__ slope,
                                                         T* __restrict__ dz, long long lddz, float* __restrict__ partial)
 {
     constexpr int N = Chunk<T>::N;
@@ -400,14 +402,14 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(long long rows, int n, i
             unpack<T>(load16_head(dy + r * lddy + col, valid), g);
             if (slope) {
                 if (valid >= N) {
-                    typename Slope<T>::type s[N];
+                    float s[N];
                     __builtin_memcpy(s, slope + r * n + col, sizeof s);
 #pragma unroll
-                    for (int i = 0; i < N; i++) g[i] *= (float)s[i];
+                    for (int i = 0; i < N; i++) g[i] *= s[i];
                 } else {
 #pragma unroll
                     for (int i = 0; i < N; i++)
-                        if (i < valid) g[i] *= (float)slope[r * n + col + i];
+                        if (i < valid) g[i] *= slope[r * n + col + i];
                 }
             }
             if (dz) store16_head(dz + r * lddz + col, pack<T>(g), lddz - col);
@@ -693,7 +695,7 @@ static BackwardPlan backward_plan(long long rows, int k, int n, int dtype, int a
 template <typename T>
 static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtype, int act, const void* x, long long ldx,
                           const void* w, long long ldw, const void* bias, const void* res, long long ldr, void* y,
-                          void* slope, char* workspace)
+                          float* slope, char* workspace)
 {
     Product<T> a = {};
     a.p = (const T*)w;
@@ -708,7 +710,7 @@ static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtyp
     a.epi.residual = (const T*)res;
     a.epi.ldr = ldr;
     a.epi.y = (T*)y;
-    a.epi.slope = act == NGS_ACT_NONE ? nullptr : (typename Slope<T>::type*)slope;
+    a.epi.slope = act == NGS_ACT_NONE ? nullptr : slope;
     a.epi.np = n;
     if (ngs_few_rows_takes(rows, k, n, dtype)) return ngs_few_rows<T>(st, rows, k, n, a.q, ldx, a.p, ldw, a.epi);
     if (ngs_stream_forward_takes(rows, k, n, dtype))
@@ -729,7 +731,7 @@ static int linear_forward(hipStream_t st, long long rows, int k, int n, int dtyp
 
 template <typename T>
 static int linear_backward(hipStream_t st, long long rows, int k, int n, int dtype, int act, const void* x, long long ldx,
-                           const void* w, long long ldw, const void* bias, const void* slope, const void* dy, long long lddy,
+                           const void* w, long long ldw, const void* bias, const float* slope, const void* dy, long long lddy,
                            void* dx, void* dw, void* db, char* workspace)
 {
     if (ngs_stream_backward_takes(rows, k, n, dtype))
@@ -744,7 +746,7 @@ static int linear_backward(hipStream_t st, long long rows, int k, int n, int dty
     if (make_dz || db) {
         const dim3 grid((unsigned)b.row_blocks, (unsigned)b.col_blocks);
         hipLaunchKernelGGL(linear_dz_kernel<T>, grid, dim3(256), 0, st, rows, n, b.across, (const T*)dy, lddy,
-                           act == NGS_ACT_NONE ? nullptr : (const typename Slope<T>::type*)slope,
+                           act == NGS_ACT_NONE ? nullptr : slope,
                            make_dz ? (T*)workspace : nullptr, b.ldz, db ? sums : nullptr);
         if (db) ngs_launch_column_finish(st, sums, b.row_blocks, n, 0, db, nullptr, dtype);
         if (ngs_decoder_launched("ngs_linear_backward")) return 1;
@@ -829,7 +831,7 @@ extern "C" size_t ngs_linear_forward_workspace_bytes(long long rows, int in_feat
 extern "C" int ngs_linear_forward(long long rows, int in_features, int out_features, int dtype, int activation,
                                   const void* x, long long x_stride, const void* weight, long long weight_stride,
                                   const void* bias, const void* residual, long long residual_stride, void* y,
-                                  void* slope, char* workspace, void* stream)
+                                  float* slope, char* workspace, void* stream)
 {
     const int k = in_features, n = out_features;
     if (check_linear("ngs_linear_forward", rows, k, n, dtype, activation)) return 1;
@@ -852,10 +854,13 @@ extern "C" int ngs_linear_forward(long long rows, int in_features, int out_featu
                                 residual_stride, y, slope, workspace);
 }
 
-extern "C" int ngs_linear_backward_reads_slope(long long rows, int in_features, int out_features, int dtype, int activation)
+extern "C" size_t ngs_linear_slope_bytes(long long rows, int in_features, int out_features, int dtype, int activation)
 {
-    if (rows <= 0 || out_features <= 0 || !ngs_decoder_dtype(dtype) || activation == NGS_ACT_NONE) return 0;
-    return ngs_stream_backward_takes(rows, in_features, out_features, dtype) ? 0 : 1;
+    if (rows <= 0 || in_features < 0 || out_features <= 0 || too_many(rows, in_features, out_features) ||
+        !ngs_decoder_dtype(dtype) || activation == NGS_ACT_NONE)
+        return 0;
+    if (ngs_stream_backward_takes(rows, in_features, out_features, dtype)) return 0;
+    return (size_t)rows * (size_t)out_features * sizeof(float);
 }
 
 extern "C" size_t ngs_linear_backward_workspace_bytes(long long rows, int in_features, int out_features, int dtype,
@@ -872,7 +877,7 @@ extern "C" size_t ngs_linear_backward_workspace_bytes(long long rows, int in_fea
 
 extern "C" int ngs_linear_backward(long long rows, int in_features, int out_features, int dtype, int activation,
                                    const void* x, long long x_stride, const void* weight, long long weight_stride,
-                                   const void* bias, const void* slope, const void* dL_dy, long long dL_dy_stride,
+                                   const void* bias, const float* slope, const void* dL_dy, long long dL_dy_stride,
                                    void* dL_dx, void* dL_dweight, void* dL_dbias, char* workspace, void* stream)
 {
     const int k = in_features, n = out_features;
@@ -881,7 +886,7 @@ extern "C" int ngs_linear_backward(long long rows, int in_features, int out_feat
     if (n == 0 || k == 0) dL_dweight = nullptr;
     if (n == 0) dL_dbias = nullptr;
     if (!dL_dx && !dL_dweight && !dL_dbias) return 0;
-    const bool reads_slope = ngs_linear_backward_reads_slope(rows, k, n, dtype, activation);
+    const bool reads_slope = ngs_linear_slope_bytes(rows, k, n, dtype, activation) > 0;
     const bool forms_z = activation != NGS_ACT_NONE && !reads_slope;
     if (((dL_dweight || forms_z) && ngs_decoder_operand("ngs_linear_backward: x", x, rows, k, x_stride)) ||
         ((dL_dx || forms_z) && ngs_decoder_operand("ngs_linear_backward: weight", weight, n, k, weight_stride)) ||

@@ -11,10 +11,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 #define NGS_FEW_ROWS 64  // rows that linear_rows.hip takes at most
 
-// Elements of the derivative array for T.
-template <typename T> struct Slope { typedef f16 type; };
-template <> struct Slope<float> { typedef float type; };
-
 // ---------------------------------------------------------------------------
 // Activations
 // ---------------------------------------------------------------------------
@@ -91,7 +87,9 @@ struct Epilogue {
     const T* residual;    // rows ldr apart, or NULL
     long long ldr;
     T* y;                 // [nq][np]
-    typename Slope<T>::type* slope;  // [nq][np] or NULL
+    // The activation's derivative [nq][np], or NULL.  In 32 bits whatever T: a saturated unit's derivative is far below
+    // what half precision holds (sigmoid' is 2e-9 at 20), and its gradient may not depend on the kernel that a width selects.
+    float* slope;
 };
 
 template <typename U>

@@ -155,7 +155,7 @@ struct StreamForward {
     long long ldx, ldw, ldr;
     int act;
     T* y;
-    typename Slope<T>::type* slope;  // or NULL
+    float* slope;  // or NULL
 };
 
 // KS: steps of four chunks that a row of x takes.  NB: groups of four chunks of the result that a workgroup computes
@@ -167,7 +167,6 @@ __global__ __launch_bounds__(THREADS) void stream_forward_kernel(StreamForward<T
 {
     constexpr int N = Chunk<T>::N, CH = KS * 4, PARTS = N / 4, COLS = NB * 4 * N;  // PARTS: fragments that make a chunk
     typedef WeightTile<T, CH> W;
-    typedef typename Slope<T>::type S;
     __shared__ __attribute__((aligned(16))) char weight[COLS * CH * 16];
     __shared__ __attribute__((aligned(16))) float bias[COLS];
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(THREADS) void stream_forward_kernel(StreamForward<T
 #pragma unroll
                     for (int e = 0; e < N; e += 4) {
                         const float four[4] = {slope[e], slope[e + 1], slope[e + 2], slope[e + 3]};
-                        if (r < a.rows && col + e < n) store4<S>(a.slope + r * a.n + n0 + col + e, four, n - col - e);
+                        if (r < a.rows && col + e < n) store4(a.slope + r * a.n + n0 + col + e, four, n - col - e);
                     }
                 } else {
                     activate<N>(a.act, z, v, nullptr);

@@ -21,7 +21,7 @@ struct DecoderApi {
     decltype(&ngs_linear_forward_workspace_bytes) linear_forward_ws = nullptr;
     decltype(&ngs_linear_forward) linear_forward = nullptr;
     decltype(&ngs_linear_backward_workspace_bytes) linear_backward_ws = nullptr;
-    decltype(&ngs_linear_backward_reads_slope) linear_reads_slope = nullptr;
+    decltype(&ngs_linear_slope_bytes) linear_slope_bytes = nullptr;
     decltype(&ngs_linear_backward) linear_backward = nullptr;
     decltype(&ngs_layer_norm_forward) norm_forward = nullptr;
     decltype(&ngs_layer_norm_backward_workspace_bytes) norm_backward_ws = nullptr;
@@ -152,11 +152,11 @@ Tensor linear_run(const Tensor& x, const Tensor& weight, const c10::optional<Ten
     Tensor b;
     if (bias.has_value()) b = vec(*bias);
     Tensor y = torch::empty(with_last(x, n), x.options().requires_grad(false));
-    if (slope) *slope = torch::empty({xr.rows, n}, y.options().dtype(dtype == NGS_FLOAT32 ? torch::kFloat32 : torch::kFloat16));
+    if (slope) *slope = torch::empty({xr.rows, n}, y.options().dtype(torch::kFloat32));
     Tensor ws = workspace_of(x, api.linear_forward_ws(xr.rows, (int)k, (int)n, dtype));
     check(api.linear_forward(xr.rows, (int)k, (int)n, dtype, act, xr.t.data_ptr(), xr.stride, wr.t.data_ptr(), wr.stride,
                              b.defined() ? b.data_ptr() : nullptr, rr.t.defined() ? rr.t.data_ptr() : nullptr, rr.stride,
-                             y.data_ptr(), slope ? slope->data_ptr() : nullptr, bytes_ptr(ws), stream_of(x)));
+                             y.data_ptr(), slope ? slope->data_ptr<float>() : nullptr, bytes_ptr(ws), stream_of(x)));
     return y;
 }
 
@@ -169,7 +169,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         int64_t rows = 1;
         for (int64_t d = 0; d + 1 < x.dim(); d++) rows *= x.size(d);
         const bool curved = act != NGS_ACT_NONE && (gx || gw || gb);
-        const bool keep = curved && api.linear_reads_slope(rows, (int)k, (int)n, dtype_of("linear", x), (int)act);
+        const bool keep = curved && api.linear_slope_bytes(rows, (int)k, (int)n, dtype_of("linear", x), (int)act) > 0;
         Tensor slope;
         Tensor y = linear_run(x, weight, bias, (int)act, residual, keep ? &slope : nullptr);
         // each product of the backward pass reads one of the two, the activation's derivative is kept or formed again from
@@ -211,7 +211,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
             Tensor ws = workspace_of(dy, api.linear_backward_ws(gr.rows, (int)k, (int)n, dtype, (int)act));
             check(api.linear_backward(gr.rows, (int)k, (int)n, dtype, (int)act, x.defined() ? xr.t.data_ptr() : nullptr,
                                       xr.stride, weight.defined() ? wr.t.data_ptr() : nullptr, wr.stride,
-                                      b.defined() ? b.data_ptr() : nullptr, slope.defined() ? slope.data_ptr() : nullptr,
+                                      b.defined() ? b.data_ptr() : nullptr, slope.defined() ? slope.data_ptr<float>() : nullptr,
                                       gr.t.data_ptr(), gr.stride, gx ? dx.data_ptr() : nullptr, gw ? dw.data_ptr() : nullptr,
                                       gb ? db.data_ptr() : nullptr, bytes_ptr(ws), stream_of(dy)));
         }
@@ -425,7 +425,7 @@ void ngs_decoder_bind(void* handle, const std::string& path)
     resolve(api.linear_forward_ws, handle, "ngs_linear_forward_workspace_bytes", path);
     resolve(api.linear_forward, handle, "ngs_linear_forward", path);
     resolve(api.linear_backward_ws, handle, "ngs_linear_backward_workspace_bytes", path);
-    resolve(api.linear_reads_slope, handle, "ngs_linear_backward_reads_slope", path);
+    resolve(api.linear_slope_bytes, handle, "ngs_linear_slope_bytes", path);
     resolve(api.linear_backward, handle, "ngs_linear_backward", path);
     resolve(api.norm_forward, handle, "ngs_layer_norm_forward", path);
     resolve(api.norm_backward_ws, handle, "ngs_layer_norm_backward_workspace_bytes", path);
