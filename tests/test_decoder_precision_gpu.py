@@ -7,7 +7,11 @@ sums is an exact zero.  So all error is the activation's evaluation in 32 bits, 
 The evaluation, counted in e = 2^-24 of what is added up (to first order; the sums below leave half as much again):
 exp(-|z|) has its argument rounded twice (2 |z| e) and its own result (2 e for an instruction good to one unit in the
 last place); a reciprocal has 2 e and the sum in it e; each further product e: sigmoid and its derivative stay within
-(2 |z| + 9) e."""
+(2 |z| + 9) e.  exp(-z^2 / 2) has its argument rounded three times (1.5 z^2 e); a polynomial of positive total with ten
+coefficients adds 2 e for each, its variable 3 e, what it approximates 1 e: Phi and the density stay within
+(1.5 z^2 + 30) e."""
+import math
+
 import pytest
 import torch
 
@@ -21,11 +25,15 @@ DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 # reduction; tiles through registers
 FORMS = {"few": (48, 64), "streamed": (300, 128), "tiles": (300, 512), "cut": (100, 1024), "registers": (200, 301)}
 # how far z goes
-RANGES = {"silu": (-24.0, 24.0), "sigmoid": (-24.0, 0.0)}
+RANGES = {"silu": (-24.0, 24.0), "sigmoid": (-24.0, 0.0), "gelu": (-12.0, 12.0)}
 
 
 def exact(z, act):
     """-> value, derivative, and what the terms that the derivative adds up come to, in 64 bits"""
+    if act == "gelu":
+        # (torch's ndtr is a sum about 1 on this device, and zero below -8.3)
+        phi, pdf = torch.erfc(-z / math.sqrt(2)) / 2, torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        return z * phi, phi + z * pdf, phi + z.abs() * pdf
     up, down = torch.sigmoid(z), torch.sigmoid(-z)
     if act == "silu":
         return z * up, up + z * up * down, up + z.abs() * up * down
@@ -46,6 +54,6 @@ def test_activations_keep_their_size(form, act, dtype):
     (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
     z = x.detach().to(F)
     value, slope, terms = exact(z, act)
-    rel = 1.5 * (2 * z.abs() + 9) * ref.E
+    rel = 1.5 * (1.5 * z * z + 30 if act == "gelu" else 2 * z.abs() + 9) * ref.E
     ref.assert_within(y, (value, ref.rounded(value, rel * value.abs(), dtype)), "y")
     ref.assert_within(dx, (slope, ref.rounded(slope, rel * terms, dtype)), "dx")
