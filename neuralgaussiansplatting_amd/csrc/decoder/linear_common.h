@@ -52,9 +52,10 @@ __device__ __forceinline__ float activate_one(float z, float& slope)
         return z * s;
     }
     if (ACT == NGS_ACT_SIGMOID) {
-        const float s = sigmoid(z);
-        slope = s * (1.0f - s);
-        return s;
+        // sigmoid' = sigmoid(z) sigmoid(-z): of the difference 1 - sigmoid(z) nothing would be left where z is large
+        const float t = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + t), s = t * r;
+        slope = s * r;
+        return z < 0.0f ? s : r;
     }
     slope = 1.0f;
     return z;

@@ -25,7 +25,7 @@ DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 # reduction; tiles through registers
 FORMS = {"few": (48, 64), "streamed": (300, 128), "tiles": (300, 512), "cut": (100, 1024), "registers": (200, 301)}
 # how far z goes
-RANGES = {"silu": (-24.0, 24.0), "sigmoid": (-24.0, 0.0), "gelu": (-12.0, 12.0)}
+RANGES = {"silu": (-24.0, 24.0), "sigmoid": (-24.0, 24.0), "gelu": (-12.0, 12.0)}
 
 
 def exact(z, act):
