@@ -50,6 +50,11 @@ void check_rows(const char* what, const Tensor& x)
     TORCH_CHECK(x.layout() == torch::kStrided, what, ": x must be a dense tensor");
     TORCH_CHECK(x.dim() >= 1, what, ": x must have at least one dimension");
     dtype_of(what, x);
+}
+
+// widths that the C entries count in 32 bits (a dropout's rows may be longer: a flat tensor is one)
+void check_width(const char* what, const Tensor& x)
+{
     TORCH_CHECK(x.size(-1) <= INT_MAX, what, ": rows are too long");
 }
 
@@ -223,6 +228,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>
               const c10::optional<Tensor>& residual)
 {
     check_rows("linear", x);
+    check_width("linear", x);
     const int act = activation_of(activation);
     check_like("linear", "weight", weight, x);
     TORCH_CHECK(weight.dim() == 2 && weight.size(1) == x.size(-1), "linear: weight must have dimensions (out_features, ",
@@ -315,6 +321,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
 Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps)
 {
     check_rows("layer_norm", x);
+    check_width("layer_norm", x);
     for (const auto* t : {&weight, &bias}) {
         if (!t->has_value()) continue;
         const char* name = t == &weight ? "weight" : "bias";
