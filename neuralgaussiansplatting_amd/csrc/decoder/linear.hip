@@ -211,8 +211,13 @@ struct TileLoader {
         for (int k = 0; k < LOADS; k++) {
             const uint32_t o = beyond ? 0x7ffffff0u : offset[k];
             const uint32_t to = __builtin_amdgcn_readfirstlane(lds + (k * WAVES + wave) * 1024);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :: "s"(to), "v"(o), "s"(rsrc) : "memory");
+            // (the compiler does not see the load in here: a scalar register of the resource that a vector instruction has
+            // just written is only safe to read five wait states later)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is reserved: nothing of the compiler's lives in it across the statement)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :: "s"(to), "v"(o), "s"(rsrc) : "memory", "m0");
+#pragma clang diagnostic pop
         }
         base += advance;
         left -= advance;

@@ -1,8 +1,11 @@
 """The C entries and the torch functions of the operators over feature rows, as far as no GPU is needed."""
 import ctypes
+import os
+import re
 
 import pytest
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LL = ctypes.c_longlong
 
 
@@ -24,3 +27,21 @@ def test_size_of_the_stored_derivative(lib):
         assert f(300, 512, 512, dtype, 0) == 0 and f(300, 64, 64, dtype, 2) == 0
         assert f(0, 512, 512, dtype, 2) == 0 and f(-1, 512, 512, dtype, 2) == 0 and f(300, 512, 0, dtype, 2) == 0
     assert f(300, 512, 512, 3, 2) == 0
+
+
+def test_assembly_names_the_registers_it_writes():
+    """Every inline assembly of the library that writes m0 says so to the compiler, which may keep a value there."""
+    csrc = os.path.join(ROOT, "neuralgaussiansplatting_amd", "csrc")
+    found = 0
+    for folder, _, names in os.walk(csrc):
+        for name in names:
+            if not name.endswith((".hip", ".h")):
+                continue
+            with open(os.path.join(folder, name)) as f:
+                text = f.read()
+            for statement in re.findall(r"\basm\b[^;]*;", text):
+                if re.search(r"\bs_mov_b32 m0\b", statement):
+                    found += 1
+                    clobbers = statement.rsplit(":", 1)[1]
+                    assert '"m0"' in clobbers, name + ": " + statement
+    assert found > 0
