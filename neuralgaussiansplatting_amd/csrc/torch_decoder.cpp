@@ -115,10 +115,12 @@ void refuse_double_backward(const char* what)
 
 // A gradient's accumulator belongs to the stream it was made on.  One that an earlier, eager graph of the same leaf keeps
 // alive would make the backward pass wait across streams, which a capture does not survive: refused here, where it can
-// still be told.
+// still be told.  (The leaf may be what the tensor is a view of: a slice of wider rows, a weight within flat parameters.)
 void check_capture(const char* what, const c10::optional<Tensor>& t)
 {
-    if (!wants_grad(t) || !t->is_leaf()) return;
+    if (!wants_grad(t)) return;
+    const Tensor leaf = t->is_leaf() || !t->is_view() ? *t : Tensor(t->_base());
+    if (!leaf.is_leaf() || !leaf.requires_grad()) return;
     const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t->device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {
@@ -126,7 +128,7 @@ void check_capture(const char* what, const c10::optional<Tensor>& t)
         return;
     }
     if (status == hipStreamCaptureStatusNone) return;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(leaf);
     if (!accumulator) return;
     const auto its = accumulator->stream();
     TORCH_CHECK(!its.has_value() || *its == stream.unwrap(), what,

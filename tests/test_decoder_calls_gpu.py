@@ -20,3 +20,34 @@ def test_dropout_of_a_long_flat_tensor(ops):
     assert torch.equal(y.detach().view(-1, 8), ops.dropout(x.detach().view(-1, 8), 0.5, 3))
     (dx,) = torch.autograd.grad(y, [x], x.detach())
     assert torch.equal(dx, y.detach())
+
+
+def test_capture_refuses_views_of_a_leaf_of_a_living_graph(ops):
+    """What holds for a leaf holds for a slice of its rows and for weights that lie in one flat parameter: the gradient
+    ends in the leaf's accumulator."""
+    flat = torch.linspace(-1, 1, 256, device=DEV).requires_grad_()
+    other = torch.ones(8, 8, device=DEV)
+    calls = [lambda: ops.linear(flat.view(16, 16)[:, 3:11], other), lambda: ops.linear(other, flat[64:128].view(8, 8)),
+             lambda: ops.layer_norm(other, flat[:8], flat[8:16]), lambda: ops.layer_norm(flat.view(32, 8)),
+             lambda: ops.dropout(flat.view(16, 16)[2:], 0.5, 1),
+             lambda: ops.dropout(other, 0.5, 1, residual=flat[:64].view(8, 8))]
+    for call in calls:
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="graph of the same tensor is alive"):
+            with torch.cuda.graph(graph):
+                torch.zeros(1, device=DEV)  # (an empty capture would warn)
+                call()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = call()
+            (d,) = torch.autograd.grad(y, [flat], torch.ones_like(y))
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            want = call()
+            assert torch.equal(y.detach(), want.detach())
+            assert torch.equal(d, torch.autograd.grad(want, [flat], torch.ones_like(want))[0])
+            del want
+        del y, d
