@@ -104,7 +104,9 @@ def render_features(viewpoint_camera, pc, decoder, pipe, bg_color, seed=0):
     # (the index map takes its place from the centres alone and has gradients for the feature vectors alone)
     xyz = pc.get_xyz.detach()
     idxmap, _, depth, feature_map = GaussianRasterizer2(raster_settings=settings)(xyz, None, xyz, pc._features)
-    dtype = next((p.dtype for p in decoder.parameters()), feature_map.dtype)
+    # (a decoder with weights gets the rows in their type, any other callable as they are)
+    weights = decoder.parameters() if isinstance(decoder, torch.nn.Module) else ()
+    dtype = next((p.dtype for p in weights), feature_map.dtype)
     colors = decoder(feature_map.to(dtype), seed).to(feature_map.dtype)
     image = torch.where((idxmap >= 0).unsqueeze(-1), colors, bg_color.to(colors.dtype))
     return {"render": image.permute(2, 0, 1), "idxmap": idxmap, "depth": depth, "feature_map": feature_map}
