@@ -105,7 +105,7 @@ def render_features(viewpoint_camera, pc, decoder, pipe, bg_color, seed=0):
     xyz = pc.get_xyz.detach()
     idxmap, _, depth, feature_map = GaussianRasterizer2(raster_settings=settings)(xyz, None, xyz, pc._features)
     # (a decoder with weights gets the rows in their type, any other callable as they are)
-    weights = decoder.parameters() if isinstance(decoder, torch.nn.Module) else ()
+    weights = getattr(decoder, "parameters", tuple)()
     dtype = next((p.dtype for p in weights), feature_map.dtype)
     colors = decoder(feature_map.to(dtype), seed).to(feature_map.dtype)
     image = torch.where((idxmap >= 0).unsqueeze(-1), colors, bg_color.to(colors.dtype))
