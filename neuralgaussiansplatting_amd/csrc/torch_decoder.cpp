@@ -385,11 +385,14 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     }
 };
 
-// a Python number as 64 bits: what exceeds them is cut off, negative ones wrap
+// a whole number (Python's, or one that says it is, as numpy's do) as 64 bits: what exceeds them is cut off, negative
+// ones wrap
 int64_t word(const char* name, const pybind11::handle& number)
 {
-    TORCH_CHECK(PyLong_Check(number.ptr()), "dropout: ", name, " must be a whole number");
-    return (int64_t)PyLong_AsUnsignedLongLongMask(number.ptr());
+    TORCH_CHECK(PyIndex_Check(number.ptr()) && !THPVariable_Check(number.ptr()), "dropout: ", name, " must be a whole number");
+    const auto whole = pybind11::reinterpret_steal<pybind11::object>(PyNumber_Index(number.ptr()));
+    if (!whole) throw pybind11::error_already_set();
+    return (int64_t)PyLong_AsUnsignedLongLongMask(whole.ptr());
 }
 
 Tensor dropout(const Tensor& x, double p, const pybind11::object& seed, const pybind11::object& offset,

@@ -1,4 +1,5 @@
 """Calls of the operators over feature rows that their documentation allows, beyond those of test_decoder_ops_gpu.py."""
+import numpy as np
 import pytest
 import torch
 
@@ -51,3 +52,19 @@ def test_capture_refuses_views_of_a_leaf_of_a_living_graph(ops):
             assert torch.equal(d, torch.autograd.grad(want, [flat], torch.ones_like(want))[0])
             del want
         del y, d
+
+
+def test_dropout_takes_whole_numbers_of_any_kind(ops):
+    """numpy's whole numbers count as Python's; what is not whole is refused, and so is a tensor as offset."""
+    x = torch.ones(500, device=DEV)
+    want = ops.dropout(x, 0.5, 7, offset=3)
+    for kind in (np.int32, np.int64, np.uint8):
+        assert torch.equal(ops.dropout(x, 0.5, kind(7), offset=kind(3)), want)
+    assert torch.equal(ops.dropout(x, 0.5, np.int64(-1)), ops.dropout(x, 0.5, -1))
+    for bad in (np.float32(7), 7.0, "7", None, [7]):
+        with pytest.raises((RuntimeError, TypeError)):
+            ops.dropout(x, 0.5, bad)
+        with pytest.raises((RuntimeError, TypeError)):
+            ops.dropout(x, 0.5, 7, offset=bad)
+    with pytest.raises(RuntimeError):
+        ops.dropout(x, 0.5, 7, offset=torch.tensor(3))
