@@ -130,3 +130,5 @@ inline int ngs_decoder_operand(const char* what, const void* p, long long rows, 
 // long, the first width0 columns going to out0, the others to out1.  A NULL output is left out.  No rows: zeros.
 void ngs_launch_column_finish(hipStream_t s, const float* partial, long long blocks, long long width0, long long width1,
                               void* out0, void* out1, int dtype);
+// That launch takes 1024 threads for 64 columns: more than it holds are refused before anything else is launched.
+inline int ngs_decoder_columns(const char* what, long long columns) { return ngs_decoder_grid(what, (columns + 63) / 64, 1024); }

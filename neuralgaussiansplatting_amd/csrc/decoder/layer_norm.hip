@@ -533,6 +533,7 @@ extern "C" int ngs_layer_norm_backward(long long rows, int width, int dtype, int
     if (width == 0 || (!dL_dx && !dL_dweight && !dL_dbias)) return 0;
     hipStream_t st = (hipStream_t)stream;
     const bool sums = dL_dweight || dL_dbias;
+    if (sums && ngs_decoder_columns(what, 2LL * width)) return 1;
     if (rows == 0) {  // sums over nothing
         if (sums) ngs_launch_column_finish(st, nullptr, 0, width, width, dL_dweight, dL_dbias, weight_dtype);
         return ngs_decoder_launched(what);

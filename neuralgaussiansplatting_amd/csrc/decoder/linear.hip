@@ -891,6 +891,7 @@ extern "C" int ngs_linear_backward(long long rows, int in_features, int out_feat
     if (n == 0 || k == 0) dL_dweight = nullptr;
     if (n == 0) dL_dbias = nullptr;
     if (!dL_dx && !dL_dweight && !dL_dbias) return 0;
+    if (dL_dbias && ngs_decoder_columns("ngs_linear_backward", n)) return 1;
     const bool reads_slope = ngs_linear_slope_bytes(rows, k, n, dtype, activation) > 0;
     const bool forms_z = activation != NGS_ACT_NONE && !reads_slope;
     if (((dL_dweight || forms_z) && ngs_decoder_operand("ngs_linear_backward: x", x, rows, k, x_stride)) ||

@@ -45,3 +45,21 @@ def test_assembly_names_the_registers_it_writes():
                     clobbers = statement.rsplit(":", 1)[1]
                     assert '"m0"' in clobbers, name + ": " + statement
     assert found > 0
+
+
+def test_column_sums_that_one_launch_does_not_hold_are_refused(lib):
+    """Widths whose gradient sums would take 2^32 threads are refused before anything is launched."""
+    some, none = ctypes.c_void_p(4096), None  # (an address that is never used)
+
+    def norm(rows, width, dw, db):
+        return lib.ngs_layer_norm_backward(LL(rows), width, 0, 0, some, LL(width), none, some, some, some, LL(width), none, dw, db,
+                                           some, none)
+
+    def linear(rows, n, db):
+        return lib.ngs_linear_backward(LL(rows), 8, n, 0, 0, some, LL(8), some, LL(8), none, none, some, LL(n), none, none, db, some,
+                                       none)
+
+    for call in (lambda: norm(4, 1 << 28, some, none), lambda: norm(4, 1 << 30, none, some), lambda: norm(0, 1 << 28, some, some),
+                 lambda: linear(4, (1 << 28) + 1, some), lambda: linear(0, 1 << 30, some)):
+        assert call() == 1
+        assert b"too many elements for one launch" in lib.ngs_last_error()
