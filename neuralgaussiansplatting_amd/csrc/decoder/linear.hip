@@ -280,11 +280,10 @@ __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&a
                 float slope[N];
                 if (a.epi.slope) {
                     activate<N>(a.epi.act, z, y, slope);
+                    // (into the place of z: its chunks are twice a result's of 16 bits, and leave below in whole lines)
 #pragma unroll
-                    for (int e = 0; e < N; e += 4) {
-                        const float four[4] = {slope[e], slope[e + 1], slope[e + 2], slope[e + 3]};
-                        if (e < valid) store4(a.epi.slope + q * a.np + p + e, four, valid - e);
-                    }
+                    for (int e = 0; e < N; e += 4)
+                        *(f32x4*)&lds[r * PITCH + col + e] = (f32x4){slope[e], slope[e + 1], slope[e + 2], slope[e + 3]};
                 } else {
                     activate<N>(a.epi.act, z, y, nullptr);
                 }
@@ -298,6 +297,19 @@ __device__ __forceinline__ void finish_wide(const Product<T>& a, const f32x4 (&a
             }
         }
         __builtin_amdgcn_wave_barrier();
+        if (!BARE && a.epi.slope) {
+            constexpr int QUADS = MP * 4;  // of a row
+#pragma unroll 1
+            for (int t = lane; t < 16 * QUADS; t += 64) {
+                const int r = t / QUADS, c = t % QUADS * 4;
+                const long long q = q0 + j * 16 + r;
+                if (q >= a.nq || p0 + c >= a.np) continue;
+                const f32x4 v = *(const f32x4*)&lds[r * PITCH + c];
+                const float four[4] = {v[0], v[1], v[2], v[3]};
+                store4(a.epi.slope + q * a.np + p0 + c, four, a.np - (int)p0 - c);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 

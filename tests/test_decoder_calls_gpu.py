@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_decoder_ops_gpu import check_linear
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
@@ -68,3 +70,10 @@ def test_dropout_takes_whole_numbers_of_any_kind(ops):
             ops.dropout(x, 0.5, 7, offset=bad)
     with pytest.raises(RuntimeError):
         ops.dropout(x, 0.5, 7, offset=torch.tensor(3))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("act", ["gelu", "sigmoid"])
+@pytest.mark.parametrize("size", [(300, 512, 515), (130, 1024, 321), (523, 520, 514)], ids=str)
+def test_stored_derivative_at_widths_that_end_inside_a_tile(ops, size, act, dtype):
+    check_linear(ops, *size, dtype, act, True, True)
