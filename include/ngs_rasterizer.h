@@ -412,10 +412,10 @@ int ngs_idxmap_forward_static(int P, int width, int height, const float* means3D
  *
  * dtype names the element type of every array typed void* unless noted.  Row strides are in elements and may be any
  * non-negative number; elements of a row are contiguous, and so are outputs, rows included.  Arrays need the
- * alignment of their element type only; a workspace needs 16 bytes.  Rows of linear and layer norm have at most 2^30 elements; what
- * a launch does not hold is refused.  Sums, statistics and activations are formed in
- * 32 bits, each output is rounded once, and results do not depend on timing (no atomics).  Sizes of zero are fine.
- * Outputs must not overlap inputs, unless noted.
+ * alignment of their element type only; a workspace needs 16 bytes.  Rows of linear and layer norm have at most 2^30
+ * elements; what a launch does not hold is refused.  Sums, statistics and activations are formed in 32 bits, each output
+ * is rounded once, and results do not depend on timing (no atomics).  Sizes of zero are fine.  Outputs must not overlap
+ * inputs, unless noted.
  *
  * ngs_linear_forward: y = act(x weight^T + bias) + residual, with x [rows][in_features] (rows x_stride apart), weight
  * [out_features][in_features] (rows weight_stride apart), bias [out_features] or NULL, residual [rows][out_features]
@@ -428,7 +428,7 @@ int ngs_idxmap_forward_static(int P, int width, int height, const float* means3D
  * ngs_linear_backward: with dz = dL_dy * slope, dL_dx = dz weight, dL_dweight = dz^T x, dL_dbias = sum of dz over the
  * rows; any of the three may be NULL.  bias as in the forward call.  dL_dy [rows][out_features], rows dL_dy_stride apart.  (A residual's gradient
  * is dL_dy itself.)  For the 16-bit types dz is rounded to the type in front of the two products, which the matrix
- * units take in that type; dL_dbias sums it unrounded.
+ * units take in that type (a float16 dz beyond 65504 becomes infinite); dL_dbias sums it unrounded.
  *
  * ngs_layer_norm_forward: y = (x - m) r weight + bias with m the mean of a row of x [rows][width] and
  * r = 1 / sqrt(variance + eps), the variance the biased one about m.  weight and bias [width] are of weight_dtype

@@ -9,7 +9,7 @@
 // rows a workgroup walks through; the workgroups' sums are joined in order by a second kernel.
 //
 // Bound by memory: 1920 x 1080 x 64 float32 there and back moves 2.65 GB (x is read by both passes) in 488 us, 5.4 TB/s;
-// 8191 x 5001 float16 410 MB in 134 us, of which rows that start off a word's boundary cost a quarter (5000 wide: 103 us).
+// 8191 x 5001 float16 410 MB in 133 us, of which rows that start off a word's boundary cost a quarter (5000 wide: 101 us).
 #include "decoder_common.h"
 
 #define NORM_WAVE_BLOCKS 1024  // workgroups of the kernels that give a row to a wave or less: what fills the chip
@@ -81,7 +81,9 @@ struct Weights {
 
 // Whether a group has its next row on the way while it works on one: worth its registers for narrow rows and for groups
 // of several waves, which stand at barriers together; a lone wave with much to hold makes room for other waves instead
-// (100000 x 1024 bfloat16 there and back: 223 us ahead, 208 us not; 8191 x 5001 float16: 144 us and 172 us).
+// (100000 x 1024 bfloat16 there and back: 223 us ahead, 208 us not; 8191 x 5001 float16: 144 us and 172 us).  Four chunks of
+// 16-bit types are more than the backward pass has registers for: 64 to 124 bytes a lane go to memory and back for every
+// row (8191 x 6144 float16 there and back 116 us, 8192 wide 188 us; 4096 x 12288 120 us, 16384 wide 240 us).
 template <int GROUP, int NC>
 constexpr bool norm_reads_ahead() { return GROUP <= 64 ? NC == 1 : GROUP < 1024; }
 

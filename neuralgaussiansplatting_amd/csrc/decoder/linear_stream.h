@@ -12,11 +12,16 @@
 // weight (dx) and, with x, through shared memory into the product over the rows (dW), whose sums stay in registers
 // until the workgroup is done.
 //
-// Measured: 640000 rows 128 -> 128 bfloat16 with gelu and residual, kernel times: forward 492 MB in 99 us (5.0 TB/s, at a
-// large copy's rate), backward 492 MB in 193 us (2.5 TB/s).  Without an activation the two together take 211 us instead
-// of 268 us, so forming z and the derivative again is about 40 us of the backward pass; 242 registers a lane leave it two
-// waves to a SIMD, too few to hide the rest under the loads.  1920 x 1080 rows 64 -> 128 float32 forward with relu moves
-// 1.59 GB in 357 us (4.5 TB/s).
+// Measured: 640000 rows 128 -> 128 bfloat16 with gelu and residual, kernel times: forward 494 MB in 103 us (4.8 TB/s, at a
+// large copy's rate), backward 509 MB in 202 us (2.5 TB/s).  Without an activation the two together take 211 us instead
+// of 280 us, of which the forward pass is 93 and 99 us: forming z and the derivative again is about 60 us of the backward
+// pass; 241 registers a lane leave it two waves to a SIMD, too few to hide it under the loads.  1920 x 1080 rows 64 -> 128
+// float32 forward with relu moves 1.59 GB in 358 us (4.5 TB/s).
+//
+// Widths count in steps of four chunks, rounded up to a power of two, and what of them is empty is left out only where
+// there is much of it: unequal and odd widths are further from the memory's rate (292504 rows 14 -> 168 bfloat16 there and
+// back 112 us for 213 MB; 893582 rows 40 -> 152 float32 926 us for 1.4 GB).  Widths of 129 to 256 beside narrow ones hold
+// one wave a SIMD, and float32 of 17 to 32 against 129 to 256 spills 348 bytes a lane (893582 rows 20 -> 152: 1658 us).
 #pragma once
 #include "linear_common.h"
 
@@ -267,8 +272,10 @@ constexpr int stream_waves(int ks, int ns, int size)
 {
     return ks * ns <= 8 || ks * ns > 32 || ks > 8 || ns > 8 || (size == 2 && (ks > 4 || ns > 4)) ? 4 : 8;
 }
-// Workgroups of a compute unit: what its registers hold, which is asked of the compiler as well, so that the launch is one
-// round and no unit works on a second while others wait (640000 rows 39 (of 64) -> 3 float32 there and back: 116 us, 133 us
+// Workgroups of a compute unit: at most what its registers hold, so that the launch is one round and no unit works on a
+// second while others wait.  A table, kept by hand with the compiler's report: it is the kernel's launch bound, so the
+// compiler makes the registers fit, and the smallest (one or two steps in all), of which five to seven would fit, stay at
+// four (640000 rows 39 (of 64) -> 3 float32 there and back: 116 us, 133 us
 // with four workgroups where three were held; 200 -> 3 bfloat16 190 us, 278 us).
 constexpr int stream_per_cu(int ks, int ns, int size)
 {
@@ -399,7 +406,7 @@ void stream_backward_kernel(StreamBackward<T> a)
                         const bool whole = (s * 4 + 4) * N <= a.n;  // uniform
 #pragma unroll
                         for (int e = 0; e < N; e++) d[e] = whole || e < left ? d[e] * slope[e] : 0.0f;
-                        dz[s] = pack<T>(d);
+                        dz[s] = pack<T>(d);  // (rounded for the matrix units: see linear_dz_kernel)
                     }
                     if constexpr (!DB_MMA) {
 #pragma unroll

@@ -6,10 +6,14 @@ rows.  All three take float32, float16 and bfloat16 tensors on the GPU with any 
 32 bits, round each output once, run on the current stream of the tensors' device, and have gradients (first ones:
 ``create_graph=True`` is refused).  Rows may lie apart (a slice of a wider map is not copied).  Results do not depend on
 timing.  The functions come straight from the compiled extension: no Python runs inside a call or its backward pass.
+They do not go through torch's dispatcher, so ``torch.autocast`` does not touch them: the tensors' own types decide, and a
+call whose tensors' types differ is refused.
 
 ``linear(x, weight, bias=None, activation="none", residual=None)``
     ``act(x @ weight.T + bias) + residual``: x [..., in], weight [out, in], bias [out], residual [..., out], all of one
-    type.  ``activation`` is "none", "relu", "gelu" (x Phi(x)), "silu" or "sigmoid".
+    type.  ``activation`` is "none", "relu", "gelu" (x Phi(x)), "silu" or "sigmoid".  With an activation, the gradients of
+    16-bit x and weight are products with dL/dz rounded to their type, which the matrix units take (the bias's gradient sums
+    it unrounded); as any float16 gradient, a dL/dz beyond 65504 is infinite.  Where that matters, use float32.
 
 ``layer_norm(x, weight=None, bias=None, eps=1e-5)``
     ``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, ``var`` the biased variance; weight and

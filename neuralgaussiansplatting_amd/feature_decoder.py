@@ -18,7 +18,8 @@ class FeatureDecoder(nn.Module):
 
     Every line but the norms is one kernel forward.  ``dropout`` is the probability while training (``train()``); the
     masks are functions of the ``seed`` given to the call, a whole number or one int64 on the GPU (see
-    ``decoder_ops.dropout``), so pass another one every step."""
+    ``decoder_ops.dropout``), so pass another one every step.  Everything runs in the type of the weights, which the features
+    must have, also under ``torch.autocast``: for 16 bits, make or convert the decoder in that type."""
 
     def __init__(self, in_features=NUM_FEATURES, width=128, blocks=2, out_features=3, dropout=0.0, device=None, dtype=None):
         super().__init__()
