@@ -1,4 +1,6 @@
 """Calls of the operators over feature rows that their documentation allows, beyond those of test_decoder_ops_gpu.py."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -77,3 +79,73 @@ def test_dropout_takes_whole_numbers_of_any_kind(ops):
 @pytest.mark.parametrize("size", [(300, 512, 515), (130, 1024, 321), (523, 520, 514)], ids=str)
 def test_stored_derivative_at_widths_that_end_inside_a_tile(ops, size, act, dtype):
     check_linear(ops, *size, dtype, act, True, True)
+
+
+def step_of(ops, g, dtype, rows, k, n):
+    """-> inputs of a training step through tiles (or padded copies) and a wide norm, and the step"""
+    make = lambda *s, scale=1.0: (torch.randn(s, generator=g, device=DEV) * scale).to(dtype)
+    x, w, b = make(rows, k).requires_grad_(), make(n, k, scale=k ** -0.5).requires_grad_(), make(n).requires_grad_()
+    dy = make(rows, n)
+
+    def step():
+        y = ops.layer_norm(ops.linear(x, w, b, activation="silu"))
+        return [y.detach(), *torch.autograd.grad(y, [x, w, b], dy)]
+
+    return (x, w, b, dy), step
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("size", [(700, 1001, 1203), (2100, 1208, 1203), (512, 512, 9000)], ids=str)
+def test_tiles_captured_and_replayed(ops, size, dtype):
+    """Two graphs in one memory pool, replayed in turn with eager work between, on new inputs each time: the bits of
+    eager steps."""
+    graphs = []
+    pool = torch.cuda.graph_pool_handle()
+    for seed in (1, 2):
+        inputs, step = step_of(ops, torch.Generator(device=DEV).manual_seed(seed), dtype, *size)
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = step()
+        graphs.append((inputs, step, graph, out))
+    g = torch.Generator(device=DEV).manual_seed(3)
+    for _ in range(3):
+        for inputs, step, graph, out in graphs:
+            with torch.no_grad():
+                for t in inputs:
+                    t.copy_(torch.randn(t.shape, generator=g, device=DEV) * 0.1)
+            graph.replay()
+            torch.cuda.synchronize()
+            kept = [t.clone() for t in out]
+            for a, b in zip(kept, step()):
+                assert torch.equal(a, b)
+
+
+def test_threads_on_streams_of_their_own(ops):
+    """Four threads, each on its own stream: the bits of a lone call."""
+    work = [step_of(ops, torch.Generator(device=DEV).manual_seed(i), dtype, *size) for i, (dtype, size) in enumerate(
+        [(torch.float32, (900, 64, 48)), (torch.bfloat16, (700, 600, 777)), (torch.float16, (40, 1000, 90)),
+         (torch.bfloat16, (3000, 39, 130))])]
+    want = [step() for _, step in work]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = work[i][1]()
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        failed.append(i)
+        except Exception as e:  # reported by the test's thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
