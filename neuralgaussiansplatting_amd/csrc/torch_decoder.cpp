@@ -406,6 +406,7 @@ Tensor dropout(const Tensor& x, double p, const pybind11::object& seed, const py
         seed_tensor = seed.cast<Tensor>();
         TORCH_CHECK(seed_tensor->scalar_type() == torch::kInt64 && seed_tensor->numel() == 1 && seed_tensor->device() == x.device(),
                     "dropout: a seed tensor must be one int64 on ", x.device().str());
+        if (seed_tensor->is_neg()) seed_tensor = seed_tensor->resolve_neg();
     } else {
         seed_word = word("seed", seed);
     }

@@ -149,3 +149,12 @@ def test_threads_on_streams_of_their_own(ops):
     for t in threads:
         t.join()
     assert not failed
+
+
+def test_dropout_reads_a_lazily_negated_seed_by_its_value(ops):
+    x = torch.ones(1000, device=DEV, requires_grad=True)
+    lazy = torch._neg_view(torch.tensor([5], device=DEV))
+    assert lazy.is_neg()
+    y = ops.dropout(x, 0.4, lazy)
+    assert torch.equal(y, ops.dropout(x, 0.4, -5))
+    assert torch.equal(torch.autograd.grad(y, [x], torch.ones_like(y))[0], y.detach())
